@@ -433,6 +433,100 @@ SB_API int sb_token_overlap(const void *donor_tokens, int32_t donor_dtype, int64
                             void *workspace, int64_t workspace_bytes, int64_t *overlap, void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* Paged cache: append, gather and attention                                */
+/* ------------------------------------------------------------------------ */
+/* No counterpart in the reference, whose engines do this part; it is what a
+ * donor-reuse step needs beside the inject: the recomputed rows go into the
+ * same paged cache, attention reads them there together with the injected
+ * rows, and a request's rows come back out as donor KV. */
+
+/* New tokens of a batch of requests.  Token t < n_tokens belongs to the
+ * request b with cu_seqlens[b] <= t < cu_seqlens[b + 1] (cu_seqlens[0] = 0,
+ * ascending; requests without tokens are fine) and stands at positions[t] of
+ * it.  Tokens at or behind cu_seqlens[batch] are padding: nothing of them is
+ * read or written.  Position p of request b lives in physical block
+ * block_tables[b * table_stride + p / block_size]; p < 0, p / block_size >=
+ * max_blocks and entries outside [0, n_blocks) address no row. */
+typedef struct sb_paged_batch {
+  const void *block_tables;  /* device, table_dtype */
+  const int32_t *cu_seqlens; /* device, batch + 1 entries */
+  const void *positions;     /* device, n_tokens entries of pos_dtype */
+  int64_t table_stride;
+  int32_t batch, n_tokens, max_blocks;
+  int32_t table_dtype, pos_dtype; /* SB_INDEX_* */
+  int32_t reserved;               /* 0 */
+} sb_paged_batch;
+
+/* One layer of a paged cache.  group == 0: rows of head_dim elements of
+ * `dtype`, row (block, kv, head, position in block) at data + the strides in
+ * elements.  group = 32, 64 or 128 (head_dim 64 or 128, a multiple of group):
+ * a cache held in 4 bits; data holds rows of head_dim / 2 bytes (element 2i in
+ * the low half of byte i; strides in bytes), scales rows of head_dim / group
+ * fp16 pairs (step, zero) (strides in fp16 elements), and element d of a row
+ * stands for zero[d / group] + code[d] * step[d / group].  4-bit caches want
+ * data, scales and their strides at multiples of 16 bytes (scales: 4 bytes). */
+typedef struct sb_paged_cache {
+  void *data;
+  void *scales;
+  int64_t stride_block, stride_kv, stride_head, stride_pos;
+  int64_t scale_block, scale_kv, scale_head, scale_pos;
+  int32_t n_blocks, block_size, n_heads, head_dim;
+  int32_t group;
+  int32_t dtype; /* SB_DTYPE_* of the cache's rows (group == 0) */
+} sb_paged_cache;
+
+/* Rows of a [tokens, heads, head_dim] tensor, head_dim contiguous; strides in
+ * elements. */
+typedef struct sb_token_rows {
+  void *data;
+  int64_t stride_token, stride_head;
+} sb_token_rows;
+
+/* Write each token's K (rotated to its position) and V row into the cache,
+ * and its rotated query rows into query_out (both query.data and
+ * query_out.data NULL: none; query_out may be query).  RoPE pair i turns by
+ * positions[t] * inv_freq[i] (device, head_dim / 2 doubles; NULL: no
+ * rotation); the angle is formed in 64 bits.  16- and 32-bit caches: rotated
+ * in fp32, one rounding to `dtype`, which is the cache's.  4-bit caches: K is
+ * rotated in 64 bits and rounded to fp32 (so that codes do not depend on the
+ * last bits of cos and sin); per group zero = fp16(min), step =
+ * fp16((max - min) / 15), code = the nearest integer to (x - zero) * (1 /
+ * step) in fp32, limited to 0..15; values beyond +-65504 saturate.  A token
+ * whose position addresses no row is not written and counted once in
+ * *err_counter (device uint64, may be NULL).  No two tokens of a call may
+ * share a row. */
+SB_API int sb_paged_append(const sb_paged_cache *cache, const sb_paged_batch *batch, sb_token_rows key,
+                           sb_token_rows value, sb_token_rows query, sb_token_rows query_out,
+                           int32_t n_q_heads, int32_t dtype, const double *inv_freq, int32_t rotary_style,
+                           uint64_t *err_counter, void *stream);
+
+/* Copy each token's K and V row out of the cache into key_out / value_out of
+ * `dtype` (the cache's own for 16- and 32-bit caches; any for 4-bit caches,
+ * whose values are rounded to it once).  Tokens whose position addresses no
+ * row are skipped and counted as by sb_paged_append. */
+SB_API int sb_paged_gather(const sb_paged_cache *cache, const sb_paged_batch *batch, sb_token_rows key_out,
+                           sb_token_rows value_out, int32_t dtype, uint64_t *err_counter, void *stream);
+
+/* Device bytes sb_paged_attention needs (16-byte aligned); -1 for invalid
+ * arguments.  One workspace serves one call at a time. */
+SB_API int64_t sb_paged_attention_workspace_bytes(const sb_paged_cache *cache, const sb_paged_batch *batch,
+                                                  int32_t n_q_heads, int32_t dtype);
+
+/* Attention of each token's query rows over its request's cached rows: key j
+ * is visible at position p when j <= p, j addresses a row and, with window >
+ * 0, j > p - window or j < sinks (window = 0: every j <= p).  Query head h
+ * reads KV head h / (n_q_heads / n_heads).  out = softmax(scale * q . k) v
+ * with fp32 statistics and accumulation; a token that sees no key gives 0.
+ * What invisible rows hold (NaN and infinities included) does not matter.
+ * `dtype` is the type of query and out, and of a 16- or 32-bit cache.
+ * *status (device int32, zeroed by the caller, may be NULL) receives a value
+ * >= 2 if a kernel wait timed out. */
+SB_API int sb_paged_attention(const sb_paged_cache *cache, const sb_paged_batch *batch, sb_token_rows query,
+                              sb_token_rows out, int32_t n_q_heads, int32_t window, int32_t sinks, float scale,
+                              int32_t dtype, void *workspace, int64_t workspace_bytes, int32_t *status,
+                              void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* Miscellaneous                                                            */
 /* ------------------------------------------------------------------------ */
 SB_API const char *sb_status_string(int status);

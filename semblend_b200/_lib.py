@@ -99,6 +99,53 @@ class SbAttnTensor(ctypes.Structure):
     ]
 
 
+class SbPagedBatch(ctypes.Structure):
+    _fields_ = [
+        ("block_tables", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("batch", ctypes.c_int32),
+        ("n_tokens", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("table_dtype", ctypes.c_int32),
+        ("pos_dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class SbPagedCache(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("stride_block", ctypes.c_int64),
+        ("stride_kv", ctypes.c_int64),
+        ("stride_head", ctypes.c_int64),
+        ("stride_pos", ctypes.c_int64),
+        ("scale_block", ctypes.c_int64),
+        ("scale_kv", ctypes.c_int64),
+        ("scale_head", ctypes.c_int64),
+        ("scale_pos", ctypes.c_int64),
+        ("n_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("group", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class SbTokenRows(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("stride_token", ctypes.c_int64),
+        ("stride_head", ctypes.c_int64),
+    ]
+
+
+# the C names of the structs above that the header declares
+C_STRUCT_NAMES = {"SbPagedBatch": "sb_paged_batch", "SbPagedCache": "sb_paged_cache", "SbTokenRows": "sb_token_rows"}
+
 _P = ctypes.POINTER
 _SIGNATURES: dict[str, tuple] = {
     "sb_inject": (ctypes.c_int, [_P(SbInjectDesc), ctypes.c_int32, _P(SbInjectParams), ctypes.c_void_p, ctypes.c_void_p]),
@@ -188,6 +235,23 @@ _SIGNATURES: dict[str, tuple] = {
         [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
          ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p],
+    ),
+    "sb_paged_append": (
+        ctypes.c_int,
+        [_P(SbPagedCache), _P(SbPagedBatch), SbTokenRows, SbTokenRows, SbTokenRows, SbTokenRows, ctypes.c_int32,
+         ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p],
+    ),
+    "sb_paged_gather": (
+        ctypes.c_int,
+        [_P(SbPagedCache), _P(SbPagedBatch), SbTokenRows, SbTokenRows, ctypes.c_int32, ctypes.c_void_p,
+         ctypes.c_void_p],
+    ),
+    "sb_paged_attention_workspace_bytes": (
+        ctypes.c_int64, [_P(SbPagedCache), _P(SbPagedBatch), ctypes.c_int32, ctypes.c_int32]),
+    "sb_paged_attention": (
+        ctypes.c_int,
+        [_P(SbPagedCache), _P(SbPagedBatch), SbTokenRows, SbTokenRows, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+         ctypes.c_float, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p],
     ),
     "sb_profile_start": (ctypes.c_int, [ctypes.c_int32]),
     "sb_profile_stop": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),

@@ -1,0 +1,172 @@
+// Attention from a paged cache: causal, with an optional sliding window and a
+// few first tokens that stay visible (sm_100a).
+//
+// Query row (token t of request b at position p, head h) sees key j when
+// j <= p, (j > p - window or j < sinks), and j's page is mapped;
+//     out = softmax(scale * q . k_j) v_j over the keys seen, 0 if there are none.
+#include <algorithm>
+#include <cmath>
+
+#include "paged.cuh"
+#include "prof.cuh"
+
+namespace sb {
+namespace {
+
+using paged::find_block;
+using paged::find_request;
+using paged::load_position;
+
+struct AttendParams {
+  sb_paged_cache cache;
+  sb_paged_batch batch;
+  sb_token_rows q, out;
+  int Hq, G;        // query heads, query heads per KV head
+  int window;       // 0x7fffffff: none
+  int sinks;
+  float scale;
+};
+
+// Keys [0, sink_end) and [first, end) are those a token at position p may see.
+struct Span {
+  int sink_end, first, end;
+};
+__device__ __forceinline__ Span key_span(const AttendParams &P, int p) {
+  const int64_t held = (int64_t)P.batch.max_blocks * P.cache.block_size;
+  Span s;
+  s.end = (int)min((int64_t)p + 1, held);
+  s.first = min(max(p - P.window, -1) + 1, s.end);  // window = 0x7fffffff gives 0
+  s.sink_end = min(P.sinks, s.first);
+  return s;
+}
+
+// One element of a cache row.
+template <typename T>
+__device__ __forceinline__ float cache_elem(const AttendParams &P, int64_t row, int64_t scale_row, int d) {
+  if (P.cache.group == 0) return Elem<T>::to_f32(reinterpret_cast<const T *>(P.cache.data)[row + d]);
+  const uint8_t c = reinterpret_cast<const uint8_t *>(P.cache.data)[row + d / 2];
+  const __half2 sz = *reinterpret_cast<const __half2 *>(reinterpret_cast<const __half *>(P.cache.scales) + scale_row +
+                                                        2 * (d / P.cache.group));
+  const float2 f = __half22float2(sz);
+  return fmaf((float)(d & 1 ? c >> 4 : c & 15), f.x, f.y);
+}
+
+// CUDA-core path (any head_dim <= 256, any type and page size): one CTA per
+// (token, query head), 128 keys at a time: a thread scores one key, then the
+// threads share the head's dimensions for P.V.  Keys that are not seen are
+// never read.
+template <typename T>
+__global__ void __launch_bounds__(128) attend_simt_kernel(const AttendParams P) {
+  const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+  const int b = find_request(P.batch, t);
+  if (b < 0) return;
+  const int D = P.cache.head_dim, g = h / P.G, bs = P.cache.block_size;
+  __shared__ float qs[256];
+  __shared__ float ps[128];
+  __shared__ int64_t vrow[128], vscale[128];
+  __shared__ float red[4];
+  const T *q = reinterpret_cast<const T *>(P.q.data) + (int64_t)t * P.q.stride_token + (int64_t)h * P.q.stride_head;
+  for (int d = tid; d < D; d += 128) qs[d] = Elem<T>::to_f32(q[d]) * P.scale;
+  __syncthreads();
+  const Span sp = key_span(P, load_position(P.batch, t));
+  float mrun = -INFINITY, lrun = 0.f, acc0 = 0.f, acc1 = 0.f;
+  const int n_sink = (sp.sink_end + 127) / 128, n = n_sink + (sp.end - sp.first + 127) / 128;
+  for (int i = 0; i < n; ++i) {
+    const int key = i < n_sink ? i * 128 + tid : sp.first + (i - n_sink) * 128 + tid;
+    const bool in = key < (i < n_sink ? sp.sink_end : sp.end);
+    const int phys = in ? find_block(P.batch, b, key / bs, P.cache.n_blocks) : -1;
+    float sc = -INFINITY;
+    vrow[tid] = -1;
+    if (phys >= 0) {
+      const int64_t in_block = key % bs;
+      const int64_t row = phys * P.cache.stride_block + in_block * P.cache.stride_pos + g * P.cache.stride_head;
+      const int64_t srow = phys * P.cache.scale_block + in_block * P.cache.scale_pos + g * P.cache.scale_head;
+      float dot = 0.f;
+      for (int d = 0; d < D; ++d) dot = fmaf(qs[d], cache_elem<T>(P, row, srow, d), dot);
+      sc = dot;
+      vrow[tid] = row + P.cache.stride_kv;
+      vscale[tid] = srow + P.cache.scale_kv;
+    }
+    float mx = sc;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if ((tid & 31) == 0) red[tid >> 5] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    __syncthreads();
+    const float m_new = fmaxf(mrun, mx);
+    const float base = m_new > -INFINITY ? m_new : 0.f;
+    const float corr = mrun > -INFINITY ? expf(mrun - base) : 0.f;
+    const float p = phys >= 0 ? expf(sc - base) : 0.f;
+    ps[tid] = p;
+    float sum = p;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((tid & 31) == 0) red[tid >> 5] = sum;
+    __syncthreads();
+    lrun = lrun * corr + (red[0] + red[1] + red[2] + red[3]);
+    acc0 *= corr, acc1 *= corr;
+    for (int j = 0; j < 128; ++j) {
+      if (vrow[j] < 0) continue;
+      if (tid < D) acc0 = fmaf(ps[j], cache_elem<T>(P, vrow[j], vscale[j], tid), acc0);
+      if (tid + 128 < D) acc1 = fmaf(ps[j], cache_elem<T>(P, vrow[j], vscale[j], tid + 128), acc1);
+    }
+    mrun = m_new;
+    __syncthreads();
+  }
+  T *o = reinterpret_cast<T *>(P.out.data) + (int64_t)t * P.out.stride_token + (int64_t)h * P.out.stride_head;
+  // lrun is 0 only if no key is seen (a NaN score gives a NaN sum)
+  if (tid < D) o[tid] = Elem<T>::from_f32(lrun == 0.f ? 0.f : acc0 / lrun);
+  if (tid + 128 < D) o[tid + 128] = Elem<T>::from_f32(lrun == 0.f ? 0.f : acc1 / lrun);
+}
+
+template <typename T>
+int launch_simt(const AttendParams &P, cudaStream_t st) {
+  const int slot = prof_before(st);
+  attend_simt_kernel<T><<<dim3((unsigned)P.batch.n_tokens, (unsigned)P.Hq), 128, 0, st>>>(P);
+  prof_after(slot, st);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace sb
+
+extern "C" SB_API int64_t sb_paged_attention_workspace_bytes(const sb_paged_cache *cache, const sb_paged_batch *batch,
+                                                             int32_t n_q_heads, int32_t dtype) {
+  using namespace sb;
+  if (paged::check_cache(cache) != SB_OK || paged::check_batch(batch) != SB_OK || n_q_heads <= 0 ||
+      n_q_heads % cache->n_heads || !elem_bytes(dtype))
+    return -1;
+  return 0;
+}
+
+extern "C" SB_API int sb_paged_attention(const sb_paged_cache *cache, const sb_paged_batch *batch,
+                                         sb_token_rows query, sb_token_rows out, int32_t n_q_heads, int32_t window,
+                                         int32_t sinks, float scale, int32_t dtype, void *workspace,
+                                         int64_t workspace_bytes, int32_t *status, void *stream) {
+  using namespace sb;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int s = paged::check_cache(cache);
+  if (s == SB_OK) s = paged::check_batch(batch);
+  if (s != SB_OK) return s;
+  if (!elem_bytes(dtype)) return SB_ERR_UNSUPPORTED;
+  if (cache->group == 0 && cache->dtype != dtype) return SB_ERR_INVALID_ARGUMENT;
+  if (n_q_heads <= 0 || n_q_heads % cache->n_heads || window < 0 || sinks < 0 || !std::isfinite(scale))
+    return SB_ERR_INVALID_ARGUMENT;
+  if (cache->head_dim > 256) return SB_ERR_UNSUPPORTED;
+  if (n_q_heads > 65535) return SB_ERR_TOO_LARGE;
+  if (batch->batch == 0 || batch->n_tokens == 0) return SB_OK;
+  if (!query.data || !out.data) return SB_ERR_INVALID_ARGUMENT;
+  AttendParams P;
+  P.cache = *cache, P.batch = *batch;
+  P.q = query, P.out = out;
+  P.Hq = n_q_heads, P.G = n_q_heads / cache->n_heads;
+  P.window = window ? window : 0x7fffffff;
+  P.sinks = window ? sinks : 0;
+  P.scale = scale;
+  switch (dtype) {
+    case SB_DTYPE_F32: return launch_simt<float>(P, st);
+    case SB_DTYPE_F16: return launch_simt<__half>(P, st);
+    default: return launch_simt<__nv_bfloat16>(P, st);
+  }
+}

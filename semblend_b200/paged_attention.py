@@ -1,0 +1,393 @@
+"""Attention from the paged cache the inject fills, and the rows around it.
+
+A donor-reuse step injects the reused rows into an engine's paged cache
+(:mod:`semblend_b200.rope_correction`) and recomputes the others.  This module
+does the rest of a layer on that same cache:
+
+* :func:`append_paged_kv` rotates the new tokens' K (and query) to their
+  positions and writes K and V into their pages;
+* :func:`paged_attention` attends from the cache: causal, any mix of requests
+  with one new token or thousands, contiguous or scattered (the recomputed rows
+  of a partial prefill), with an optional sliding window and a few first
+  tokens that stay visible (sinks);
+* :func:`gather_paged_kv` reads rows back as donor KV, the ``[2, H, S, D]``
+  that :func:`~semblend_b200.rope_correction.inject_donors` takes.
+
+All three take either a per-layer cache tensor (float32, float16 or bfloat16,
+in any of the layouts of the inject) or an :class:`Int4KVCache`, which holds
+the same rows in 4 bits with a step and a zero per group of 32, 64 or 128
+elements.  They run on the tensors' device and its current stream, never
+synchronise, and can be captured into a CUDA graph.  There is no CPU path:
+host tensors raise :class:`~semblend_b200._lib.NativeLibraryError`.
+
+The reference leaves this part to the serving engine, so it has no counterpart
+there.
+"""
+
+from __future__ import annotations
+
+import math
+from contextlib import nullcontext
+
+import torch
+
+from . import _lib, _rows
+
+INT4_GROUPS = (32, 64, 128)
+INT4_HEAD_DIMS = (64, 128)
+
+_freqs: dict[tuple, torch.Tensor] = {}
+
+
+def _need(t, name: str, device: torch.device | None = None) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    _lib.require_cuda(t, name)
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _on(device: torch.device):
+    """The device's context, entered only where it is not the current one."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _inv_freq64(rope_base: float, head_dim: int, device: torch.device) -> torch.Tensor:
+    """``base ** (-2i / D)`` in 64 bits, built once per (base, head_dim, device)."""
+    key = (float(rope_base), head_dim, device.index)
+    t = _freqs.get(key)
+    if t is None:
+        host = float(rope_base) ** (-torch.arange(0, head_dim, 2, dtype=torch.float64) / head_dim)
+        t = _freqs[key] = host.to(device)
+    return t
+
+
+class PagedBatch:
+    """The new tokens of a step: which request each belongs to and where it stands.
+
+    ``block_tables`` ``[B, max_blocks]`` (int32 / int64) maps each request's
+    logical blocks to physical ones (entries a request does not use may hold
+    anything outside ``[0, num_blocks)``, such as -1); ``cu_seqlens`` ``[B + 1]``
+    (int32, ascending from 0) gives request ``b`` the tokens ``cu_seqlens[b] ..
+    cu_seqlens[b + 1] - 1``, possibly none; ``positions`` ``[T]`` (int32 /
+    int64) their positions in their request, in any order.  Tokens at or behind
+    ``cu_seqlens[-1]`` are padding.  One batch serves every layer of a step;
+    the tensors are read when the kernels run, so a captured graph follows
+    what they then hold.
+    """
+
+    __slots__ = ("block_tables", "cu_seqlens", "positions", "device", "_c")
+
+    def __init__(self, block_tables: torch.Tensor, cu_seqlens: torch.Tensor, positions: torch.Tensor):
+        _need(block_tables, "block_tables")
+        dev = block_tables.device
+        _need(cu_seqlens, "cu_seqlens", dev)
+        _need(positions, "positions", dev)
+        if block_tables.ndim != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+            raise ValueError(f"block_tables must be [B, max_blocks] with contiguous rows, got {tuple(block_tables.shape)}")
+        if cu_seqlens.dtype != torch.int32:
+            raise TypeError(f"cu_seqlens must be int32, got {cu_seqlens.dtype}")
+        if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] != block_tables.shape[0] + 1 or not cu_seqlens.is_contiguous():
+            raise ValueError(f"cu_seqlens must be a contiguous [{block_tables.shape[0] + 1}] tensor, got {tuple(cu_seqlens.shape)}")
+        if positions.ndim != 1 or not positions.is_contiguous():
+            raise ValueError(f"positions must be a contiguous 1-D tensor, got {tuple(positions.shape)}")
+        self.block_tables, self.cu_seqlens, self.positions, self.device = block_tables, cu_seqlens, positions, dev
+        c = _lib.SbPagedBatch()
+        c.block_tables = block_tables.data_ptr()
+        c.cu_seqlens = cu_seqlens.data_ptr()
+        c.positions = positions.data_ptr()
+        c.batch, c.max_blocks = block_tables.shape
+        c.table_stride = block_tables.stride(0) if c.batch > 1 else c.max_blocks
+        if c.table_stride < c.max_blocks:
+            raise ValueError("the rows of block_tables overlap")
+        c.n_tokens = positions.shape[0]
+        c.table_dtype = _lib.index_code(block_tables.dtype)
+        c.pos_dtype = _lib.index_code(positions.dtype)
+        self._c = c
+
+    @property
+    def n_tokens(self) -> int:
+        return self._c.n_tokens
+
+
+class Int4KVCache:
+    """A paged cache (one layer) held in 4 bits.
+
+    ``codes`` is the cache's per-layer shape with ``D / 2`` bytes per row
+    (uint8, element ``2i`` in the low half of byte ``i``), ``scales`` the same
+    with ``[D / group, 2]`` float16 pairs ``(step, zero)`` in place of the row:
+    element ``d`` stands for ``zero + code * step`` of its group.  ``layout`` is
+    one of the layouts of the 16-bit caches.
+    """
+
+    __slots__ = ("codes", "scales", "layout", "group", "head_dim", "device", "_c")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, *, layout: str = "canonical"):
+        _need(codes, "codes")
+        _need(scales, "scales", codes.device)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.float16:
+            raise TypeError(f"codes must be uint8 and scales float16, got {codes.dtype} and {scales.dtype}")
+        if layout not in _rows.LAYOUTS:
+            raise ValueError(f"unknown KV layout {layout!r}; expected one of {_rows.LAYOUTS}")
+        nb, nh, bs, half = _rows.paged_geometry(codes.shape, layout)
+        if scales.ndim != 6 or scales.shape[:4] != codes.shape[:4] or scales.shape[5] != 2 or scales.shape[4] < 1:
+            raise ValueError(f"scales {tuple(scales.shape)} do not match codes {tuple(codes.shape)}")
+        self.codes, self.scales, self.layout, self.device = codes, scales, layout, codes.device
+        self.head_dim, self.group = 2 * half, 2 * half // scales.shape[4]
+        if self.head_dim not in INT4_HEAD_DIMS or self.group not in INT4_GROUPS or self.group * scales.shape[4] != self.head_dim:
+            raise ValueError(
+                f"a 4-bit cache holds rows of {INT4_HEAD_DIMS} elements in groups of {INT4_GROUPS}; got {self.head_dim} "
+                f"elements in {scales.shape[4]} groups"
+            )
+        if codes.stride(4) != 1 or scales.stride(5) != 1 or (scales.shape[4] > 1 and scales.stride(4) != 2):
+            raise ValueError("the rows of codes and scales must be contiguous")
+        c = _lib.SbPagedCache()
+        c.data, c.scales = codes.data_ptr(), scales.data_ptr()
+        c.stride_block, c.stride_kv, c.stride_head, c.stride_pos = _axis_strides(codes, layout)
+        c.scale_block, c.scale_kv, c.scale_head, c.scale_pos = _axis_strides(scales, layout)
+        c.n_blocks, c.block_size, c.n_heads, c.head_dim, c.group = nb, bs, nh, self.head_dim, self.group
+        self._c = c
+
+    @classmethod
+    def allocate(cls, num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int, *, group: int = 64,
+                 layout: str = "canonical", device: torch.device | str = "cuda") -> Int4KVCache:
+        """An empty cache (every row stands for zeros)."""
+        if layout not in _rows.LAYOUTS:
+            raise ValueError(f"unknown KV layout {layout!r}; expected one of {_rows.LAYOUTS}")
+        if head_dim not in INT4_HEAD_DIMS or group not in INT4_GROUPS or group > head_dim:
+            raise ValueError(f"head_dim must be one of {INT4_HEAD_DIMS} and group one of {INT4_GROUPS}, at most head_dim; "
+                             f"got {head_dim} and {group}")
+        sizes = {"canonical": (num_blocks, 2, num_kv_heads, block_size), "vllm": (2, num_blocks, block_size, num_kv_heads),
+                 "trtllm": (num_blocks, 2, block_size, num_kv_heads)}[layout]
+        if torch.device(device).type != "cuda":
+            raise _lib.NativeLibraryError(f"a 4-bit cache lives on a CUDA device, not on {device}")
+        return cls(torch.zeros(*sizes, head_dim // 2, dtype=torch.uint8, device=device),
+                   torch.zeros(*sizes, head_dim // group, 2, dtype=torch.float16, device=device), layout=layout)
+
+    @property
+    def num_kv_heads(self) -> int:
+        return self._c.n_heads
+
+
+def _axis_strides(t: torch.Tensor, layout: str) -> tuple[int, int, int, int]:
+    """(block, kv, head, position) strides; a dimension of one element may carry any, so it gets 0."""
+    shape, stride = t.shape, t.stride()
+    return tuple(0 if shape[a] == 1 else stride[a] for a in _rows._AXES[layout][:4])
+
+
+def _cache(kv_cache, batch: PagedBatch, layout: str) -> _lib.SbPagedCache:
+    if isinstance(kv_cache, Int4KVCache):
+        if layout not in ("auto", kv_cache.layout):
+            raise ValueError(f"the cache is laid out as {kv_cache.layout!r}, not {layout!r}")
+        if kv_cache.device != batch.device:
+            raise ValueError(f"kv_cache is on {kv_cache.device}, expected {batch.device}")
+        return kv_cache._c
+    _need(kv_cache, "kv_cache", batch.device)
+    layout = _rows.resolve_layout(kv_cache, layout)
+    nb, nh, bs, hd = _rows.paged_geometry(kv_cache.shape, layout)
+    if hd > 1 and kv_cache.stride(4) != 1:
+        raise ValueError("the rows of kv_cache must be contiguous")
+    c = _lib.SbPagedCache()
+    c.data, c.scales, c.group = kv_cache.data_ptr(), None, 0
+    c.stride_block, c.stride_kv, c.stride_head, c.stride_pos = _axis_strides(kv_cache, layout)
+    c.n_blocks, c.block_size, c.n_heads, c.head_dim = nb, bs, nh, hd
+    c.dtype = _lib.dtype_code(kv_cache.dtype)
+    return c
+
+
+def _token_rows(t: torch.Tensor, name: str, batch: PagedBatch, heads: int | None, head_dim: int,
+                dtype: torch.dtype | None = None) -> _lib.SbTokenRows:
+    """A ``[T, heads, D]`` tensor with contiguous rows."""
+    _need(t, name, batch.device)
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != batch._c.n_tokens or shape[2] != head_dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} must be [{batch._c.n_tokens}, {'heads' if heads is None else heads}, {head_dim}], "
+                         f"got {tuple(shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} dtype {t.dtype} differs from {dtype}")
+    st = t.stride()
+    if st[2] != 1 and head_dim > 1:
+        raise ValueError(f"the rows of {name} must be contiguous")
+    return _lib.SbTokenRows(t.data_ptr(), 0 if shape[0] == 1 else st[0], 0 if shape[1] == 1 else st[1])
+
+
+def _written(t: torch.Tensor, name: str) -> None:
+    """An output whose rows lie on one another has no one answer."""
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        raise ValueError(f"{name} is expanded: its rows share memory")
+
+
+_NO_ROWS = _lib.SbTokenRows()
+
+
+def append_paged_kv(
+    kv_cache: torch.Tensor | Int4KVCache,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    batch: PagedBatch,
+    rope_base: float | None = 10000.0,
+    *,
+    query: torch.Tensor | None = None,
+    query_out: torch.Tensor | None = None,
+    rotary_style: str = "interleaved",
+    layout: str = "auto",
+) -> torch.Tensor | Int4KVCache:
+    """Write the batch's K, rotated to its positions, and V into the paged cache.
+
+    ``key`` / ``value`` are ``[T, H, D]`` before the rotation (any token and
+    head strides, so slices of a fused projection do) in the cache's dtype; a
+    4-bit cache takes any of the three dtypes and quantises each row by its
+    groups.  ``rope_base=None`` writes K as it is.  With ``query``
+    ``[T, Hq, D]`` its rotated rows are written to ``query_out``, which may be
+    ``query`` itself.  Angles are formed in 64 bits, so far positions keep
+    their fraction of a turn.  A token whose position lies outside its
+    request's mapped blocks is skipped and counted
+    (:func:`semblend_b200.skipped_pairs`); padding is left alone.  No two
+    tokens of a call may share a (page, offset).  Modified in place and
+    returned.
+    """
+    c = _cache(kv_cache, batch, layout)
+    dtype = key.dtype if isinstance(kv_cache, Int4KVCache) else kv_cache.dtype
+    code = _lib.dtype_code(dtype)
+    hd = c.head_dim
+    if hd % 2 or hd > 512:
+        raise ValueError(f"head_dim must be even and at most 512, got {hd}")
+    k = _token_rows(key, "key", batch, c.n_heads, hd, dtype)
+    v = _token_rows(value, "value", batch, c.n_heads, hd, dtype)
+    if (query is None) != (query_out is None):
+        raise ValueError("query and query_out come together")
+    q = qo = _NO_ROWS
+    hq = 0
+    if query is not None:
+        q = _token_rows(query, "query", batch, None, hd, dtype)
+        hq = query.shape[1]
+        qo = _token_rows(query_out, "query_out", batch, hq, hd, dtype)
+        _written(query_out, "query_out")
+        if hq == 0:
+            q = qo = _NO_ROWS
+    style = _rows.rotary_code(rotary_style)
+    dev = batch.device
+    freq = None if rope_base is None else _inv_freq64(rope_base, hd, dev).data_ptr()
+    with _on(dev):
+        _lib.check(
+            _lib.load().sb_paged_append(c, batch._c, k, v, q, qo, hq, code, freq, style,
+                                        _lib.err_counter(dev).data_ptr(), _lib.stream_ptr(dev)),
+            "append_paged_kv",
+        )
+    return kv_cache
+
+
+def gather_paged_kv(
+    kv_cache: torch.Tensor | Int4KVCache,
+    batch: PagedBatch,
+    *,
+    out: torch.Tensor | None = None,
+    dtype: torch.dtype | None = None,
+    layout: str = "auto",
+) -> torch.Tensor:
+    """Read the batch's rows out of the cache as donor KV ``[2, H, T, D]``.
+
+    The result feeds :class:`~semblend_b200.rope_correction.DonorInjection`
+    (its positions are the tokens' indices) and
+    :func:`~semblend_b200.rope_correction.rope_correct_scatter_paged`; K is as
+    the cache holds it, rotated to where it stood.  ``dtype`` (default: the
+    cache's; bfloat16 for a 4-bit cache) must be the cache's own unless it is
+    held in 4 bits.  Tokens without a row are skipped and counted; their rows
+    and padding stay as they were in ``out``, and zero in a new result.
+    """
+    c = _cache(kv_cache, batch, layout)
+    four = isinstance(kv_cache, Int4KVCache)
+    if dtype is None:
+        dtype = out.dtype if out is not None else torch.bfloat16 if four else kv_cache.dtype
+    if not four and dtype != kv_cache.dtype:
+        raise TypeError(f"dtype {dtype} differs from kv_cache dtype {kv_cache.dtype}")
+    code = _lib.dtype_code(dtype)
+    dev = batch.device
+    if out is None:
+        out = torch.zeros(2, c.n_heads, batch._c.n_tokens, c.head_dim, dtype=dtype, device=dev)
+    else:
+        _need(out, "out", dev)
+        if out.ndim != 4 or out.shape[0] != 2:
+            raise ValueError(f"out must be [2, {c.n_heads}, {batch._c.n_tokens}, {c.head_dim}], got {tuple(out.shape)}")
+        _written(out, "out")
+    k, v = (_token_rows(out[i].transpose(0, 1), "out", batch, c.n_heads, c.head_dim, dtype) for i in (0, 1))
+    with _on(dev):
+        _lib.check(
+            _lib.load().sb_paged_gather(c, batch._c, k, v, code, _lib.err_counter(dev).data_ptr(), _lib.stream_ptr(dev)),
+            "gather_paged_kv",
+        )
+    return out
+
+
+def paged_attention(
+    query: torch.Tensor,
+    kv_cache: torch.Tensor | Int4KVCache,
+    batch: PagedBatch,
+    *,
+    window: int | None = None,
+    sinks: int = 0,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+    layout: str = "auto",
+    status: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Causal attention of the batch's query rows over their cached rows.
+
+    ``query`` / ``out`` are ``[T, Hq, D]`` (``Hq`` a multiple of the cache's
+    heads; query head h reads KV head ``h // (Hq // H)``) in the cache's dtype,
+    or any of the three over a 4-bit cache.  The token at position ``p`` sees
+    key ``j`` when ``j <= p``, its block is mapped and, with ``window``,
+    ``j > p - window`` or ``j < sinks``.  The new tokens' own rows must be in
+    the cache first (:func:`append_paged_kv`).  Softmax statistics and sums are
+    fp32.  A token that sees no key gives zeros; what unseen rows hold (NaN
+    and infinities included) has no effect.  Padding rows stay as they were in
+    ``out``, and zero in a new result.  ``status`` (device int32) receives a
+    value >= 2 if a kernel wait timed out.
+    """
+    c = _cache(kv_cache, batch, layout)
+    _need(query, "query", batch.device)
+    dtype = query.dtype if isinstance(kv_cache, Int4KVCache) else kv_cache.dtype
+    code = _lib.dtype_code(dtype)
+    hd = c.head_dim
+    q = _token_rows(query, "query", batch, None, hd, dtype)
+    hq = query.shape[1]
+    if hq == 0 or hq % c.n_heads:
+        raise ValueError(f"{hq} query heads are not a multiple of {c.n_heads} KV heads")
+    if window is not None and not 0 < window < 1 << 31:
+        raise ValueError(f"window must be positive and below 2^31, got {window}")
+    if not 0 <= sinks < 1 << 31:
+        raise ValueError(f"sinks must not be negative and below 2^31, got {sinks}")
+    if scale is None:
+        scale = 1.0 / math.sqrt(hd)
+    elif not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    dev = batch.device
+    if out is None:
+        out = torch.zeros(query.shape, dtype=dtype, device=dev)
+    else:
+        _written(out, "out")
+    o = _token_rows(out, "out", batch, hq, hd, dtype)
+    if status is not None:
+        _need(status, "status", dev)
+        if status.dtype != torch.int32 or status.numel() < 1:
+            raise TypeError("status must be an int32 tensor of one element")
+    lib = _lib.load()
+    with _on(dev):
+        nbytes = lib.sb_paged_attention_workspace_bytes(c, batch._c, hq, code)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
+        _lib.check(
+            lib.sb_paged_attention(c, batch._c, q, o, hq, window or 0, sinks, scale, code,
+                                   None if ws is None else ws.data_ptr(), nbytes,
+                                   None if status is None else status.data_ptr(), _lib.stream_ptr(dev)),
+            "paged_attention",
+        )
+    return out
+
+
+__all__ = [
+    "Int4KVCache",
+    "PagedBatch",
+    "append_paged_kv",
+    "gather_paged_kv",
+    "paged_attention",
+]

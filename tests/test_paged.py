@@ -1,0 +1,212 @@
+"""Paged-cache operators without a GPU: addressing (compiled for the host),
+the C entry points' argument checks, and the plain restatement's own sanity."""
+
+from __future__ import annotations
+
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+from oracle import paged as op
+from semblend_b200 import _lib
+from semblend_b200 import paged_attention as pa
+
+ROOT = Path(__file__).resolve().parents[1]
+
+ADDRESSING = r"""
+#include <stdio.h>
+#include <stdint.h>
+#include "paged.cuh"
+using namespace sb::paged;
+namespace sb { void set_last_cuda_error(cudaError_t) {} }
+#define CHECK(x) do { if (!(x)) { printf("line %d: %s\n", __LINE__, #x); return 1; } } while (0)
+int main() {
+  // five requests: 0 and 3 idle, a table of 64-bit entries with a row stride
+  int32_t cu[] = {0, 0, 3, 4, 4, 9};
+  int64_t tab[5 * 4];
+  for (int i = 0; i < 20; ++i) tab[i] = i % 4 == 3 ? 99999 : i;  // the stride's gap is never an entry
+  int64_t pos[] = {0, -7, 1LL << 40, 47, 48, 3, 2, 1, 0, 5, 5};
+  sb_paged_batch B = {};
+  B.block_tables = tab, B.cu_seqlens = cu, B.positions = pos;
+  B.table_stride = 4, B.batch = 5, B.n_tokens = 11, B.max_blocks = 3;
+  B.table_dtype = SB_INDEX_I64, B.pos_dtype = SB_INDEX_I64;
+  const int owner[] = {1, 1, 1, 2, 4, 4, 4, 4, 4, -1, -1, -1};
+  for (int t = 0; t < 12; ++t) CHECK(find_request(B, t) == owner[t]);
+  B.n_tokens = 6;  // sequences that claim more tokens than there are
+  CHECK(find_request(B, 5) == 4 && find_request(B, 6) == -1 && find_request(B, 8) == -1);
+  B.n_tokens = 11;
+  int32_t odd[] = {0, 5, 2, 7, 1, 9};  // not ascending: still an index inside the batch
+  B.cu_seqlens = odd;
+  for (int t = 0; t < 11; ++t) CHECK(find_request(B, t) >= -1 && find_request(B, t) < 5);
+  B.cu_seqlens = cu;
+  CHECK(find_block(B, 2, 0, 20) == 8 && find_block(B, 2, 2, 20) == 10);
+  CHECK(find_block(B, 2, 3, 20) == -1 && find_block(B, 2, -1, 20) == -1 && find_block(B, 2, 1LL << 40, 20) == -1);
+  CHECK(find_block(B, 2, 2, 10) == -1 && find_block(B, 2, 1, 10) == 9);
+  tab[5] = -1, tab[6] = (1LL << 32) + 3;  // not 3: entries are compared in 64 bits
+  CHECK(find_block(B, 1, 1, 20) == -1 && find_block(B, 1, 2, 20) == -1);
+  CHECK(load_position(B, 1) == -1 && load_position(B, 2) == 0x7fffff00 && load_position(B, 3) == 47);
+  int32_t small[] = {0, 1, 2, -1};
+  B.block_tables = small, B.table_dtype = SB_INDEX_I32, B.batch = 1, B.max_blocks = 4, B.table_stride = 4;
+  CHECK(find_block(B, 0, 2, 3) == 2 && find_block(B, 0, 3, 3) == -1 && find_block(B, 0, 2, 2) == -1);
+  B.max_blocks = 0, B.block_tables = nullptr;
+  CHECK(find_block(B, 0, 0, 3) == -1);
+  printf("ok\n");
+  return 0;
+}
+"""
+
+
+def test_addressing_on_the_host(tmp_path):
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not Path(nvcc).exists():
+        pytest.skip("no nvcc")
+    src, exe = tmp_path / "addressing.cu", tmp_path / "addressing"
+    src.write_text(ADDRESSING)
+    subprocess.run([nvcc, "-std=c++17", f"-I{ROOT / 'semblend_b200' / 'csrc'}", str(src), "-o", str(exe)], check=True,
+                   capture_output=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert res.returncode == 0, res.stdout
+
+
+def _structs(group=0):
+    c = _lib.SbPagedCache(data=256, scales=512 if group else None, stride_block=4096, stride_kv=2048, stride_head=1024,
+                          stride_pos=64, scale_block=256, scale_kv=128, scale_head=64, scale_pos=4, n_blocks=10,
+                          block_size=16, n_heads=2, head_dim=128, group=group, dtype=_lib.SB_DTYPE_BF16)
+    b = _lib.SbPagedBatch(block_tables=256, cu_seqlens=256, positions=256, table_stride=4, batch=2, n_tokens=3,
+                          max_blocks=4, table_dtype=0, pos_dtype=0)
+    return c, b
+
+
+def _calls(c, b, **kw):
+    """Status of each entry point; the pointers are never followed: every call here is refused or empty."""
+    lib = _lib.load()
+    a = dict(key=256, q=256, out=256, hq=4, window=0, sinks=0, scale=1.0, dtype=_lib.SB_DTYPE_BF16, style=0, freq=256)
+    a.update(kw)
+    row = lambda p: _lib.SbTokenRows(p, 128, 128)  # noqa: E731
+    return {
+        "append": lib.sb_paged_append(c, b, row(a["key"]), row(a["key"]), row(a["q"]), row(a["out"]), a["hq"], a["dtype"],
+                                      a["freq"], a["style"], None, None),
+        "gather": lib.sb_paged_gather(c, b, row(a["out"]), row(a["out"]), a["dtype"], None, None),
+        "attention": lib.sb_paged_attention(c, b, row(a["q"]), row(a["out"]), a["hq"], a["window"], a["sinks"], a["scale"],
+                                            a["dtype"], None, 0, None, None),
+    }
+
+
+INV, UNS = _lib.SB_ERR_INVALID_ARGUMENT, _lib.SB_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("group", [0, 64])
+def test_entry_points_refuse_bad_geometry(group):
+    def expect(status, c_kw=None, b_kw=None, only=None, **kw):
+        c, b = _structs(group)
+        for k, v in (c_kw or {}).items():
+            setattr(c, k, v)
+        for k, v in (b_kw or {}).items():
+            setattr(b, k, v)
+        got = _calls(c, b, **kw)
+        for name in only or got:
+            assert got[name] == status, (name, got[name], c_kw, b_kw, kw)
+
+    expect(INV, {"block_size": 0})
+    expect(INV, {"n_heads": 0})
+    expect(INV, {"head_dim": 0})
+    expect(INV, {"n_blocks": -1})
+    expect(INV, {"data": None})
+    expect(INV, b_kw={"batch": -1})
+    expect(INV, b_kw={"n_tokens": -1})
+    expect(INV, b_kw={"cu_seqlens": None})
+    expect(INV, b_kw={"positions": None})
+    expect(INV, b_kw={"block_tables": None})
+    expect(INV, b_kw={"table_dtype": 2})
+    expect(INV, b_kw={"pos_dtype": -1})
+    expect(INV, b_kw={"table_stride": 3})
+    expect(UNS, dtype=7)
+    expect(INV, only=["append"], style=2)
+    expect(INV, only=["append"], key=None)
+    expect(INV, only=["append", "gather", "attention"], out=None)
+    expect(INV, only=["append", "attention"], q=None)
+    expect(INV, only=["append", "attention"], hq=0)
+    expect(INV, only=["attention"], hq=3)
+    expect(INV, only=["attention"], window=-1)
+    expect(INV, only=["attention"], sinks=-1)
+    expect(INV, only=["attention"], scale=float("inf"))
+    if group == 0:
+        expect(UNS, {"dtype": 9})
+        expect(INV, dtype=_lib.SB_DTYPE_F16)  # not the cache's
+        expect(UNS, {"head_dim": 258}, only=["attention"])
+        expect(UNS, {"head_dim": 127}, only=["append"])
+        expect(UNS, {"head_dim": 514}, only=["append"])
+    else:
+        expect(UNS, {"head_dim": 96})
+        expect(UNS, {"group": 48})
+        expect(UNS, {"group": 128, "head_dim": 64})
+        expect(INV, {"scales": None})
+        expect(UNS, {"data": 264})
+        expect(UNS, {"stride_pos": 72})
+        expect(UNS, {"scale_head": 63})
+    expect(_lib.SB_OK, b_kw={"n_tokens": 0})
+    expect(_lib.SB_OK, b_kw={"batch": 0})
+
+
+def test_workspace_size_refuses_what_the_call_refuses():
+    lib = _lib.load()
+    c, b = _structs()
+    assert lib.sb_paged_attention_workspace_bytes(c, b, 4, _lib.SB_DTYPE_BF16) >= 0
+    assert lib.sb_paged_attention_workspace_bytes(c, b, 3, _lib.SB_DTYPE_BF16) == -1
+    assert lib.sb_paged_attention_workspace_bytes(c, b, 4, 5) == -1
+    c.block_size = 0
+    assert lib.sb_paged_attention_workspace_bytes(c, b, 4, _lib.SB_DTYPE_BF16) == -1
+    assert lib.sb_paged_append(None, b, *[_lib.SbTokenRows()] * 4, 0, 2, None, 0, None, None) == INV
+    assert lib.sb_paged_append(c, None, *[_lib.SbTokenRows()] * 4, 0, 2, None, 0, None, None) == INV
+
+
+def test_host_tensors_raise():
+    tables, cu, pos = torch.zeros(1, 2, dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(_lib.NativeLibraryError):
+        pa.PagedBatch(tables, cu, pos)
+    with pytest.raises(_lib.NativeLibraryError):
+        pa.Int4KVCache(torch.zeros(2, 2, 1, 16, 32, dtype=torch.uint8), torch.zeros(2, 2, 1, 16, 1, 2, dtype=torch.float16))
+    with pytest.raises(_lib.NativeLibraryError):
+        pa.Int4KVCache.allocate(2, 1, 16, 64, device="cpu")
+    with pytest.raises(TypeError):
+        pa.PagedBatch([[0]], cu, pos)
+
+
+def test_inverse_frequencies_are_64_bit():
+    t = pa._inv_freq64(1e6, 128, torch.device("cpu"))
+    assert t.dtype == torch.float64 and t.shape == (64,) and float(t[0]) == 1.0
+    assert float(t[32]) == pytest.approx(1e-3, rel=1e-14)
+
+
+def test_quantised_rows_stay_within_half_a_step():
+    x = torch.randn(50, 3, 128, generator=torch.Generator().manual_seed(0)).double()
+    for group in (32, 64, 128):
+        codes, scales = op.quantise(x, group)
+        step = scales[..., 0].double().repeat_interleave(group, -1)
+        zero = scales[..., 1].double().repeat_interleave(group, -1)
+        # half a step, and where rounding step and zero to fp16 cut the range short, that much more
+        slack = (15 * step + zero.abs()) * 2.0**-11
+        assert torch.all((op.values(codes, scales) - x).abs() <= step / 2 + slack + 1e-6)
+        assert torch.equal(op.unpack(op.pack(codes)), codes)
+    for layout in op.AXES:
+        t = torch.arange(2 * 2 * 3 * 4 * 5).view(2, 2, 3, 4, 5)
+        assert torch.equal(op.from_layout(op.to_layout(t, layout), layout), t)
+
+
+def test_plain_attention_agrees_with_the_dense_oracle():
+    from oracle import attention as dense
+
+    g = torch.Generator().manual_seed(1)
+    q, kv = torch.randn(40, 4, 16, generator=g), torch.randn(6, 2, 2, 8, 16, generator=g).double()
+    tables = torch.tensor([[4, 0, 5, 2, 1]])
+    out, _, _ = op.attention(q, kv, tables, [0, 40], torch.arange(40))
+    flat = kv[tables[0]].transpose(0, 1).transpose(1, 2).flatten(2, 3)  # [2, H, 40, D]
+    want = dense.partial_prefill_attention(
+        q.transpose(0, 1).float(), dense.expand_kv_heads(flat[0].float(), 4), dense.expand_kv_heads(flat[1].float(), 4),
+        torch.ones(40, dtype=torch.bool))
+    assert (out.transpose(0, 1) - want.double()).abs().max() < 1e-5
+    near, _, _ = op.attention(q, kv, tables, [0, 40], torch.arange(40), window=1)
+    assert torch.allclose(near[:, 0], flat[1, 0].double())  # one key: its value
