@@ -7,38 +7,18 @@
 #include <algorithm>
 #include <cmath>
 
-#include "paged.cuh"
+#include "paged_attend.cuh"
 #include "prof.cuh"
 
 namespace sb {
 namespace {
 
+using paged::AttendParams;
 using paged::find_block;
 using paged::find_request;
+using paged::key_span;
 using paged::load_position;
-
-struct AttendParams {
-  sb_paged_cache cache;
-  sb_paged_batch batch;
-  sb_token_rows q, out;
-  int Hq, G;        // query heads, query heads per KV head
-  int window;       // 0x7fffffff: none
-  int sinks;
-  float scale;
-};
-
-// Keys [0, sink_end) and [first, end) are those a token at position p may see.
-struct Span {
-  int sink_end, first, end;
-};
-__device__ __forceinline__ Span key_span(const AttendParams &P, int p) {
-  const int64_t held = (int64_t)P.batch.max_blocks * P.cache.block_size;
-  Span s;
-  s.end = (int)min((int64_t)p + 1, held);
-  s.first = min(max(p - P.window, -1) + 1, s.end);  // window = 0x7fffffff gives 0
-  s.sink_end = min(P.sinks, s.first);
-  return s;
-}
+using paged::Span;
 
 // One element of a cache row.
 template <typename T>
@@ -137,7 +117,11 @@ extern "C" SB_API int64_t sb_paged_attention_workspace_bytes(const sb_paged_cach
   if (paged::check_cache(cache) != SB_OK || paged::check_batch(batch) != SB_OK || n_q_heads <= 0 ||
       n_q_heads % cache->n_heads || !elem_bytes(dtype))
     return -1;
-  return 0;
+  if (batch->batch == 0 || batch->n_tokens == 0) return 0;
+  paged::AttendParams P = {};
+  P.cache = *cache, P.batch = *batch;
+  P.Hq = n_q_heads, P.G = n_q_heads / cache->n_heads;
+  return paged::decode_takes(P, dtype) ? paged::decode_workspace_bytes(P) : 0;
 }
 
 extern "C" SB_API int sb_paged_attention(const sb_paged_cache *cache, const sb_paged_batch *batch,
@@ -164,6 +148,11 @@ extern "C" SB_API int sb_paged_attention(const sb_paged_cache *cache, const sb_p
   P.window = window ? window : 0x7fffffff;
   P.sinks = window ? sinks : 0;
   P.scale = scale;
+  if (paged::decode_takes(P, dtype)) {
+    if (!workspace || workspace_bytes < paged::decode_workspace_bytes(P) || !paged::multiple(workspace, 16))
+      return SB_ERR_WORKSPACE_TOO_SMALL;
+    return paged::launch_decode(P, dtype, workspace, st);
+  }
   switch (dtype) {
     case SB_DTYPE_F32: return launch_simt<float>(P, st);
     case SB_DTYPE_F16: return launch_simt<__half>(P, st);

@@ -1,0 +1,941 @@
+// Paged attention for few query rows per request: decode, speculative
+// verification, short chunks (sm_100a).
+//
+// A tile is up to R = 8 or 16 query rows of one KV group (its heads at one or
+// a few tokens); the keys a tile sees are read once for all of them.  The work
+// of a call, every (tile, KV head)'s blocks of keys in one line, is cut into
+// equal pieces, one per CTA, wherever the cuts fall: contexts of any mix of
+// lengths fill the GPU evenly and no length is needed on the host.  A tile cut
+// by a border leaves partial sums (fp32, with their running maximum and sum) in
+// the workspace and a second kernel joins them in CTA order; whole tiles are
+// written at once.
+//
+// A CTA is four warps that each take a quarter of every block and run on their
+// own (own ring of stages filled with cp.async, own running maximum and sum,
+// joined through shared memory at the end of the tile), so no barrier stands
+// between a load and its use.  The products are mma.sync m16n8k16 with the keys
+// as rows, S^T = K Q^T and O^T = V^T P^T: eight query rows then fill the
+// instruction's n = 8 instead of half of its m = 16, and the statistics of a
+// query row and its column of O^T lie in the same lanes.  The path is bound by
+// HBM, not by the products: 16 keys of head_dim 128 are 8 KB and 16 products a
+// warp, so the rate of the warp-level instruction is enough, and its register
+// operands take 4-bit codes without a trip through shared memory.
+#include <algorithm>
+#include <type_traits>
+
+#include "paged_attend.cuh"
+#include "prof.cuh"
+#include "tcgen05.cuh"
+
+namespace sb {
+namespace paged {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kMaxRequests = 1024;  // of one launch: their prefix sums lie in shared memory
+
+// Keys a warp takes at a time, stages of its ring and bytes of one stage.
+template <int D, int GROUP> struct Ring {
+  static constexpr int kKeys = GROUP == 0 ? 16 : 32;
+  static constexpr int kBlock = kKeys * kWarps;
+  static constexpr int kStages = GROUP == 0 ? (D == 128 ? 3 : 5) : 4;
+  static constexpr int kRow = GROUP == 0 ? D * 2 : D / 2;  // bytes of a row
+  // code rows are 16 bytes apart beyond their length: eight rows then start in different banks
+  static constexpr int kPitch = GROUP == 0 ? kRow : kRow + 16;
+  static constexpr int kScale = GROUP == 0 ? 0 : 4 * (D / (GROUP == 0 ? D : GROUP));  // bytes of a row's scales
+  static constexpr int kTile = kKeys * (kPitch + kScale);  // K or V of a stage
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kWarp = kStages * kStage;
+};
+
+constexpr int kRowPad = 4;  // floats between rows of the join buffer
+template <int D, int GROUP, int NT> constexpr int ring_bytes() {
+  return std::max(kWarps * Ring<D, GROUP>::kWarp, kWarps * 8 * NT * (D + kRowPad) * 4);
+}
+template <int D, int GROUP, int NT> constexpr int smem_bytes() {
+  return ring_bytes<D, GROUP, NT>() + (kMaxRequests + 1) * 8 + kWarps * 8 * 4 + kWarps * 8 * NT * 8 + 64;
+}
+
+// What CTA k leaves for the kernel that joins: the unit its range starts in.
+struct CutUnit {
+  int64_t start, end;  // blocks of the unit in the call's line of blocks
+  int64_t total;
+  int n_ctas;
+  int tok, n_tok, head, n_heads;  // head: first query head of the tile
+  int pad;
+};
+
+struct DecodeParams {
+  AttendParams a;
+  CutUnit *cuts;    // [grid]
+  float *partials;  // [grid][2][R * (D + 2)]
+  int tokens_per_tile, heads_per_tile, head_tiles;
+  int dtype;
+};
+
+// First block of CTA k.
+__host__ __device__ __forceinline__ int64_t cut_at(int64_t total, int n_ctas, int k) {
+  return total / n_ctas * k + total % n_ctas * k / n_ctas;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+template <int N> __device__ __forceinline__ void cp_async_small(uint32_t dst, const void *src, bool take) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(take ? N : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// c += A(16 x 16) B(16 x 8), fp32 accumulation.
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t *>(&v);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t x) { return __half22float2(*reinterpret_cast<__half2 *>(&x)); }
+__device__ __forceinline__ float2 unpack_bf2(uint32_t x) {
+  return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x) {
+  return std::is_same<T, __nv_bfloat16>::value ? unpack_bf2(x) : unpack_half2(x);
+}
+
+__device__ __forceinline__ float load_any(const void *p, int64_t i, int dtype) {
+  if (dtype == SB_DTYPE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]);
+  return __half2float(reinterpret_cast<const __half *>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void *p, int64_t i, float x, int dtype) {
+  if (dtype == SB_DTYPE_BF16) reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
+  else reinterpret_cast<__half *>(p)[i] = __float2half_rn(x);
+}
+
+// Address of the row of `key` in request b's pages, or false if it has none.
+__device__ __forceinline__ bool key_row(const AttendParams &P, int b, int key, int64_t &row, int64_t &scale_row) {
+  const int bs = P.cache.block_size, lb = key / bs;
+  const int phys = find_block(P.batch, b, lb, P.cache.n_blocks);
+  if (phys < 0) return false;
+  const int64_t in = key - lb * bs;
+  row = phys * P.cache.stride_block + in * P.cache.stride_pos;
+  scale_row = phys * P.cache.scale_block + in * P.cache.scale_pos;
+  return true;
+}
+
+// One element of a row of the cache (K rows; V rows lie stride_kv behind).
+template <int GROUP>
+__device__ __forceinline__ float row_elem(const AttendParams &P, int64_t row, int64_t scale_row, int d, int dtype) {
+  if (GROUP == 0) return load_any(P.cache.data, row + d, dtype);
+  const uint8_t c = reinterpret_cast<const uint8_t *>(P.cache.data)[row + d / 2];
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(
+      reinterpret_cast<const __half *>(P.cache.scales) + scale_row + 2 * (d / (GROUP == 0 ? 1 : GROUP))));
+  return fmaf((float)(d & 1 ? c >> 4 : c & 15), f.x, f.y);
+}
+
+// The rows of a tile whose sums came out infinite or NaN although a product
+// with a probability of zero may be why (a key another row of the tile sees
+// holds an infinity or a NaN): the same sums over keys [from blocks i0 to i1)
+// that this row sees, one warp a row.  Rare, and not fast.
+template <int D, int GROUP>
+__device__ __noinline__ void redo_row(const DecodeParams &P, const TileKeys &tk, int b, int g, int i0, int i1, int p,
+                                      const void *q, float *o, float *m_out, float *l_out) {
+  constexpr int KB = Ring<D, GROUP>::kBlock;
+  const AttendParams &A = P.a;
+  const int lane = threadIdx.x % 32;
+  const Span sp = key_span(A, p);
+  constexpr int kPer = D / 32;
+  float qv[kPer], acc[kPer], m = -INFINITY, l = 0.f;
+  for (int i = 0; i < kPer; ++i) qv[i] = load_any(q, lane + 32 * i, P.dtype), acc[i] = 0.f;
+  const float c = A.scale * 1.4426950408889634f;
+  for (int i = i0; i < i1; ++i)
+    for (int k = 0; k < KB; ++k) {
+      const int key = block_key(tk, i, KB) + k;
+      int64_t row, srow;
+      if (p < 0 || !in_span(sp, key) || !key_row(A, b, key, row, srow)) continue;
+      row += (int64_t)g * A.cache.stride_head, srow += (int64_t)g * A.cache.scale_head;
+      float dot = 0.f;
+      for (int j = 0; j < kPer; ++j) dot = fmaf(qv[j], row_elem<GROUP>(A, row, srow, lane + 32 * j, P.dtype), dot);
+      for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
+      const float x = dot * c, m_new = fmaxf(m, x), base = m_new > -INFINITY ? m_new : 0.f;
+      const float corr = m > -INFINITY ? exp2f(m - base) : 0.f, w = exp2f(x - base);
+      m = m_new, l = l * corr + w;
+      for (int j = 0; j < kPer; ++j)
+        acc[j] = fmaf(w, row_elem<GROUP>(A, row + A.cache.stride_kv, srow + A.cache.scale_kv, lane + 32 * j, P.dtype),
+                      acc[j] * corr);
+    }
+  for (int i = 0; i < kPer; ++i) o[lane + 32 * i] = acc[i];
+  if (lane == 0) *m_out = m, *l_out = l;
+}
+
+template <typename T, int D, int GROUP, int NT>
+__global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) {
+  using R = Ring<D, GROUP>;
+  // products of codes run in fp16, which holds them exactly; rows in their own type
+  using M = typename std::conditional<GROUP == 0, T, __half>::type;
+  constexpr int kRows = 8 * NT;
+  constexpr int KB = R::kBlock, WK = R::kKeys, SUB = WK / 16;
+  constexpr int NG = GROUP == 0 ? 1 : D / (GROUP == 0 ? D : GROUP);
+  constexpr int MT = D / 16;
+  const AttendParams &A = P.a;
+  extern __shared__ __align__(128) uint8_t smem[];
+  int64_t *prefix = reinterpret_cast<int64_t *>(smem + ring_bytes<D, GROUP, NT>());
+  uint32_t *seen_bits = reinterpret_cast<uint32_t *>(prefix + kMaxRequests + 1);  // [warp][8 stages]
+  float *stat_m = reinterpret_cast<float *>(seen_bits + kWarps * 8);             // [warp][kRows]
+  float *stat_l = stat_m + kWarps * kRows;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, r = lane / 4, q4 = lane % 4;
+  const int B = A.batch.batch, Hkv = A.cache.n_heads, bs = A.cache.block_size;
+
+  // The call's line of blocks: request by request, in it KV head by KV head, in that tile by tile.
+  for (int b = tid; b < B; b += kThreads) {
+    int lo, hi;
+    request_tokens(A.batch, b, lo, hi);
+    int64_t n = 0;
+    for (int t = lo; t < hi; t += P.tokens_per_tile)
+      n += tile_keys(A, t, min(P.tokens_per_tile, hi - t), KB).n_blocks;
+    prefix[b + 1] = n * P.head_tiles * Hkv;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int64_t carry = 0;
+    for (int b0 = 0; b0 < B; b0 += 32) {
+      int64_t x = b0 + lane < B ? prefix[b0 + lane + 1] : 0;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (b0 + lane < B) prefix[b0 + lane + 1] = carry + x;
+      carry += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) prefix[0] = 0;
+  }
+  __syncthreads();
+  const int64_t total = prefix[B];
+  const int n_ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, total));
+  int64_t cur = cut_at(total, n_ctas, blockIdx.x);
+  const int64_t stop = (int)blockIdx.x < n_ctas ? cut_at(total, n_ctas, blockIdx.x + 1) : cur;
+  const int64_t begin = cur;
+  if (cur >= stop) {
+    if (tid == 0) P.cuts[blockIdx.x].n_ctas = 0;
+    return;
+  }
+
+  const uint32_t ring = tc::smem_u32(smem) + warp * R::kWarp;
+  const uint8_t *ring_ptr = smem + warp * R::kWarp;
+  const float sl2 = A.scale * 1.4426950408889634f;
+
+  while (cur < stop) {
+    // ---- the unit that block `cur` belongs to
+    int b = 0;
+    {
+      int lo = 0, hi = B;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[mid] <= cur) lo = mid;
+        else hi = mid;
+      }
+      b = lo;
+    }
+    int tlo, thi;
+    request_tokens(A.batch, b, tlo, thi);
+    const int64_t per_head = (prefix[b + 1] - prefix[b]) / Hkv;
+    const int g = (int)((cur - prefix[b]) / per_head);
+    int64_t at = prefix[b] + g * per_head;
+    int tok = tlo, ntok = 0, ht = 0;
+    TileKeys tk;
+    for (;;) {
+      ntok = min(P.tokens_per_tile, thi - tok);
+      tk = tile_keys(A, tok, ntok, KB);
+      const int64_t span = (int64_t)tk.n_blocks * P.head_tiles;
+      if (cur < at + span) {
+        ht = (int)((cur - at) / tk.n_blocks);
+        at += (int64_t)ht * tk.n_blocks;
+        break;
+      }
+      at += span;
+      tok += P.tokens_per_tile;
+    }
+    const int i0 = (int)(cur - at);
+    const int i1 = (int)min((int64_t)tk.n_blocks, i0 + (stop - cur));
+    const int head0 = g * A.G + ht * P.heads_per_tile;
+    const int nheads = min(P.heads_per_tile, A.G - ht * P.heads_per_tile);
+    if (cur == begin && tid == 0) {
+      CutUnit c;
+      c.start = at, c.end = at + tk.n_blocks, c.total = total, c.n_ctas = n_ctas;
+      c.tok = tok, c.n_tok = ntok, c.head = head0, c.n_heads = nheads, c.pad = 0;
+      P.cuts[blockIdx.x] = c;
+    }
+    // tile row -> (token, head): row = token * heads_per_tile + head
+    auto row_place = [&](int row, int &t, int &h) -> bool {
+      const int pi = row / P.heads_per_tile, hh = row - pi * P.heads_per_tile;
+      t = tok + pi, h = head0 + hh;
+      return pi < ntok && hh < nheads;
+    };
+    int prow[NT][2];  // positions of this lane's rows of S^T (unused rows: as the last token, never stored)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        int t, h;
+        prow[nt][e] = row_place(nt * 8 + 2 * q4 + e, t, h) ? load_position(A.batch, t) : tk.pmax;
+      }
+
+    // ---- queries as the B operand of S^T: lane holds row nt * 8 + r
+    uint32_t qf[NT][MT][2];
+    float row_scale[NT][2];    // scores to log2 units, rows 2 q4 + {0, 1}
+    float qsum[NT][2][NG];     // 4-bit: sum of the row's queries over each group, in the units of the products
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      int t, h;
+      const bool live = row_place(nt * 8 + r, t, h);
+      const char *qp = reinterpret_cast<const char *>(A.q.data) +
+                       2 * ((int64_t)(live ? t : 0) * A.q.stride_token + (int64_t)(live ? h : 0) * A.q.stride_head);
+      if constexpr (GROUP == 0) {
+#pragma unroll
+        for (int ks = 0; ks < MT; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            qf[nt][ks][e] = live ? *reinterpret_cast<const uint32_t *>(qp + 2 * (16 * ks + 8 * e + 2 * q4)) : 0u;
+        row_scale[nt][0] = row_scale[nt][1] = sl2;
+      } else {
+        // Lane q4 takes, of each group, the words (8 codes) its K words hold; the word's halves are
+        // (d, d + 4) pairs.  The row is brought to a largest magnitude in [2^11, 2^12) by a power of two,
+        // which bf16 and fp16 queries survive unrounded in fp16 (what is 2^-26 of the largest may not).
+        constexpr int kWords = D / 32, WPG = GROUP / 32;
+        uint32_t raw[kWords][4];
+        float big = 0.f, sum[NG];
+#pragma unroll
+        for (int gq = 0; gq < NG; ++gq) sum[gq] = 0.f;
+#pragma unroll
+        for (int wd = 0; wd < kWords; ++wd) {
+          const int d0 = 8 * ((wd / WPG) * (GROUP / 8) + q4 * WPG + wd % WPG);
+          uint4 v = live ? *reinterpret_cast<const uint4 *>(qp + 2 * d0) : make_uint4(0, 0, 0, 0);
+          raw[wd][0] = v.x, raw[wd][1] = v.y, raw[wd][2] = v.z, raw[wd][3] = v.w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = P.dtype == SB_DTYPE_BF16 ? unpack_bf2(raw[wd][i]) : unpack_half2(raw[wd][i]);
+            big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+            sum[wd / WPG] += f.x + f.y;
+          }
+        }
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        int e = (int)((__float_as_uint(big) >> 23) & 255) - 127;  // floor(log2(big)) for normal values
+        e = big > 0.f ? min(max(e, -110), 110) : 0;
+        const float norm = __uint_as_float((uint32_t)(11 - e + 127) << 23);  // 2^(11 - e)
+#pragma unroll
+        for (int wd = 0; wd < kWords; ++wd) {
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = P.dtype == SB_DTYPE_BF16 ? unpack_bf2(raw[wd][i]) : unpack_half2(raw[wd][i]);
+            f[2 * i] = v.x * norm, f[2 * i + 1] = v.y * norm;
+          }
+          // codes 1, 3, 5, 7 of a word enter the products 16 times as large
+          qf[nt][2 * wd][0] = pack2<__half>(f[0], f[4]);
+          qf[nt][2 * wd][1] = pack2<__half>(f[1] * 0.0625f, f[5] * 0.0625f);
+          qf[nt][2 * wd + 1][0] = pack2<__half>(f[2], f[6]);
+          qf[nt][2 * wd + 1][1] = pack2<__half>(f[3] * 0.0625f, f[7] * 0.0625f);
+        }
+        // sums over the group's lanes, then from the lane of row n to the lanes of columns 2 q4 + {0, 1}
+        const float unit = norm * 0x1p-24f;
+#pragma unroll
+        for (int gq = 0; gq < NG; ++gq) {
+          sum[gq] += __shfl_xor_sync(0xffffffffu, sum[gq], 1);
+          sum[gq] += __shfl_xor_sync(0xffffffffu, sum[gq], 2);
+          qsum[nt][0][gq] = __shfl_sync(0xffffffffu, sum[gq] * unit, 4 * (2 * q4));
+          qsum[nt][1][gq] = __shfl_sync(0xffffffffu, sum[gq] * unit, 4 * (2 * q4 + 1));
+        }
+        const float back = sl2 * __uint_as_float((uint32_t)(e - 11 + 127) << 23);  // scores in units of 2^-24 norm
+        row_scale[nt][0] = __shfl_sync(0xffffffffu, back, 4 * (2 * q4)) * 0x1p24f;
+        row_scale[nt][1] = __shfl_sync(0xffffffffu, back, 4 * (2 * q4 + 1)) * 0x1p24f;
+      }
+    }
+
+    // ---- loads: this warp's keys of block i into stage s
+    const char *kbase = reinterpret_cast<const char *>(A.cache.data) +
+                        (int64_t)g * A.cache.stride_head * (GROUP == 0 ? 2 : 1);
+    const int64_t v_off = A.cache.stride_kv * (GROUP == 0 ? 2 : 1);
+    const char *sbase = reinterpret_cast<const char *>(A.cache.scales) + (int64_t)g * A.cache.scale_head * 2;
+    const bool whole_pages = bs % WK == 0;  // a warp's keys then lie in one page
+    auto page_of = [&](int i) -> int {
+      return i < i1 ? find_block(A.batch, b, (block_key(tk, i, KB) + warp * WK) / bs, A.cache.n_blocks) : -1;
+    };
+    int next_page = whole_pages ? page_of(i0) : -1;
+    auto issue = [&](int i, int s) {
+      if (i < i1) {
+        const int key0 = block_key(tk, i, KB) + warp * WK;
+        const uint32_t dst = ring + s * R::kStage;
+        bool in = lane < WK && in_span(tk.span, key0 + lane);
+        int64_t row = 0, srow = 0;  // bytes, of the lane's key (or of key0 where pages are whole)
+        if (whole_pages) {
+          const int page = next_page;
+          next_page = page_of(i + 1);  // its latency passes behind this block's work
+          in = in && page >= 0;
+          const int64_t off = key0 % bs;
+          const int64_t pg = max(page, 0);
+          row = pg * A.cache.stride_block + off * A.cache.stride_pos;
+          srow = pg * A.cache.scale_block + off * A.cache.scale_pos;
+        } else if (in) {
+          in = key_row(A, b, key0 + lane, row, srow);
+        }
+        const uint32_t bits = __ballot_sync(0xffffffffu, in);
+        if (lane == 0) seen_bits[warp * 8 + s] = bits;
+        constexpr int kChunks = R::kRow / 16;  // 16-byte pieces of a row
+        const int c = lane % kChunks;
+        constexpr int kRowsAt = 32 / kChunks;  // rows of one instruction
+#pragma unroll
+        for (int it = 0; it < WK / kRowsAt; ++it) {
+          const int rr = it * kRowsAt + lane / kChunks;
+          int64_t off;
+          if (whole_pages) off = row + rr * A.cache.stride_pos;
+          else off = __shfl_sync(0xffffffffu, row, rr);
+          const char *src = kbase + off * (GROUP == 0 ? 2 : 1) + c * 16;
+          const bool take = (bits >> rr) & 1;
+          // rows: 16-byte pieces exchanged by the row's low bits, so that eight rows of one column
+          // (ldmatrix) lie in different banks
+          const uint32_t to = dst + rr * R::kPitch + (GROUP == 0 ? ((c ^ (rr & 7)) << 4) : (c << 4));
+          cp_async16(to, take ? src : kbase, take);
+          cp_async16(to + R::kTile, take ? src + v_off : kbase, take);
+        }
+        if constexpr (GROUP != 0) {
+          const int64_t off = whole_pages ? srow + lane * A.cache.scale_pos : srow;
+          const char *src = sbase + off * 2;
+          const uint32_t to = dst + WK * R::kPitch + lane * R::kScale;
+          cp_async_small<R::kScale>(to, in ? src : sbase, in);
+          cp_async_small<R::kScale>(to + R::kTile, in ? src + A.cache.scale_kv * 2 : sbase, in);
+        }
+      }
+      cp_commit();
+    };
+
+    float o[MT][NT][4];
+    float m_run[NT][2], l_run[NT][2], z_run[NT][2][NG];  // z: sum of probability * zero (4-bit V)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m_run[nt][e] = -INFINITY, l_run[nt][e] = 0.f;
+#pragma unroll
+        for (int gq = 0; gq < NG; ++gq) z_run[nt][e][gq] = 0.f;
+      }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[mt][nt][i] = 0.f;
+
+#pragma unroll
+    for (int s = 0; s < R::kStages - 1; ++s) issue(i0 + s, s);
+    int stage = 0;
+    for (int i = i0; i < i1; ++i) {
+      cp_wait<R::kStages - 2>();
+      __syncwarp();
+      {
+        int s = stage + R::kStages - 1;
+        issue(i + R::kStages - 1, s >= R::kStages ? s - R::kStages : s);
+      }
+      const int key0 = block_key(tk, i, KB) + warp * WK;
+      const uint32_t bits = seen_bits[warp * 8 + stage];
+      const uint32_t kt = ring + stage * R::kStage, vt = kt + R::kTile;
+      const uint8_t *kp = ring_ptr + stage * R::kStage, *vp = kp + R::kTile;
+      const int last = key0 + WK - 1;
+      const bool all_seen = bits == (WK == 32 ? 0xffffffffu : (1u << (WK & 31)) - 1) && last <= tk.pmin &&
+                            (key0 > tk.pmax - A.window || last < A.sinks);
+      // ---- S^T: [SUB][NT] tiles of 16 keys x 8 rows
+      float sc[SUB][NT][4];
+#pragma unroll
+      for (int j = 0; j < SUB; ++j) {
+        if constexpr (GROUP == 0) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sc[j][nt][x] = 0.f;
+          const int mat = lane / 8, krow = (mat & 1) * 8 + (lane & 7);
+#pragma unroll
+          for (int ks = 0; ks < MT; ++ks) {
+            uint32_t a[4];
+            ldsm4(a, kt + krow * R::kPitch + (((2 * ks + (mat >> 1)) ^ (krow & 7)) << 4));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma<M>(sc[j][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+          }
+        } else {
+          // codes enter as fp16 subnormals: code * 2^-24 is the bit pattern `code`, so a mask is the conversion
+          constexpr int WPG = GROUP / 32;
+          const uint8_t *row0 = kp + (16 * j + r) * R::kPitch, *row1 = row0 + 8 * R::kPitch;
+          float2 s0[NG], s1[NG];
+#pragma unroll
+          for (int gq = 0; gq < NG; ++gq) {
+            s0[gq] = unpack_half2(*reinterpret_cast<const uint32_t *>(kp + WK * R::kPitch + (16 * j + r) * R::kScale + 4 * gq));
+            s1[gq] = unpack_half2(*reinterpret_cast<const uint32_t *>(kp + WK * R::kPitch + (16 * j + r + 8) * R::kScale + 4 * gq));
+          }
+#pragma unroll
+          for (int gq = 0; gq < NG; ++gq) {
+            float dot[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) dot[nt][x] = 0.f;
+            uint32_t w0[WPG], w1[WPG];
+            const int at_word = 4 * (gq * (GROUP / 8) + q4 * WPG);
+#pragma unroll
+            for (int e = 0; e < WPG; ++e) {
+              w0[e] = *reinterpret_cast<const uint32_t *>(row0 + at_word + 4 * e);
+              w1[e] = *reinterpret_cast<const uint32_t *>(row1 + at_word + 4 * e);
+            }
+#pragma unroll
+            for (int e = 0; e < WPG; ++e) {
+              const uint32_t x0 = w0[e] >> 8, x1 = w1[e] >> 8;
+              const uint32_t a[4] = {w0[e] & 0x000F000Fu, w1[e] & 0x000F000Fu, w0[e] & 0x00F000F0u, w1[e] & 0x00F000F0u};
+              const uint32_t c[4] = {x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u};
+              const int wd = gq * WPG + e;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma<M>(dot[nt], a, qf[nt][2 * wd][0], qf[nt][2 * wd][1]);
+                mma<M>(dot[nt], c, qf[nt][2 * wd + 1][0], qf[nt][2 * wd + 1][1]);
+              }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float2 sz = x < 2 ? s0[gq] : s1[gq];
+                const float z = gq == 0 ? sz.y * qsum[nt][x & 1][gq] : fmaf(sz.y, qsum[nt][x & 1][gq], sc[j][nt][x]);
+                sc[j][nt][x] = fmaf(sz.x, dot[nt][x], z);
+              }
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < SUB; ++j)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sc[j][nt][x] *= row_scale[nt][x & 1];
+      if (!all_seen) {
+#pragma unroll
+        for (int j = 0; j < SUB; ++j)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int kk = 16 * j + r + 8 * (x >> 1), key = key0 + kk, p = prow[nt][x & 1];
+              const bool see = ((bits >> kk) & 1) && key <= p && (key > p - A.window || key < A.sinks);
+              if (!see) sc[j][nt][x] = -INFINITY;
+            }
+      }
+      // ---- running maximum, probabilities, sums
+      float pr[SUB][NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < SUB; ++j) mx = fmaxf(mx, fmaxf(sc[j][nt][e], sc[j][nt][e + 2]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float m_old = m_run[nt][e], m_new = fmaxf(m_old, mx);
+          const float base = m_new > -INFINITY ? m_new : 0.f;
+          if (__any_sync(0xffffffffu, m_new > m_old)) {
+            const float corr = tc::ex2_approx(m_old - base);  // 0 at the first key seen
+            l_run[nt][e] *= corr;
+#pragma unroll
+            for (int gq = 0; gq < NG; ++gq) z_run[nt][e][gq] *= corr;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) o[mt][nt][e] *= corr, o[mt][nt][e + 2] *= corr;
+          }
+          m_run[nt][e] = m_new;
+#pragma unroll
+          for (int j = 0; j < SUB; ++j)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float p = tc::ex2_approx(sc[j][nt][e + 2 * y] - base);
+              pr[j][nt][e + 2 * y] = p;
+              l_run[nt][e] += p;
+            }
+        }
+      // ---- O^T += V^T P^T
+#pragma unroll
+      for (int j = 0; j < SUB; ++j) {
+        if constexpr (GROUP == 0) {
+          uint32_t pb[NT][2], pl[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float p0 = pr[j][nt][2 * y], p1 = pr[j][nt][2 * y + 1];
+              const uint32_t h = pack2<M>(p0, p1);
+              pb[nt][y] = transpose8x8(h);
+              // what 16 bits drop of a probability enters as a second product: the path waits for memory,
+              // and the one rounding would cost as much accuracy as the rounding of the result
+              const float2 f = unpack2<M>(h);
+              pl[nt][y] = transpose8x8(pack2<M>(p0 - f.x, p1 - f.y));
+            }
+          const int mat = lane / 8, vrow = (mat >> 1) * 8 + (lane & 7);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            uint32_t a[4];
+            ldsm4_trans(a, vt + vrow * R::kPitch + (((2 * mt + (mat & 1)) ^ (vrow & 7)) << 4));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma<M>(o[mt][nt], a, pb[nt][0], pb[nt][1]);
+              mma<M>(o[mt][nt], a, pl[nt][0], pl[nt][1]);
+            }
+          }
+        } else {
+          // probability * step of the key's group as the B operand, the codes of V as subnormals in A.
+          // Its rounding to fp16 moves the result by up to 2^-11 of step * code, which is two to three
+          // times the value it stands for (the zero takes the rest back): far below a bf16 result's
+          // rounding, but above an fp16 one's, for which what was dropped enters as a second product.
+          uint32_t pb[NT][NG][2], pl[NT][NG][2];
+          const bool fine = P.dtype == SB_DTYPE_F16;
+#pragma unroll
+          for (int gq = 0; gq < NG; ++gq) {
+            const float2 s0 = unpack_half2(*reinterpret_cast<const uint32_t *>(vp + WK * R::kPitch + (16 * j + r) * R::kScale + 4 * gq));
+            const float2 s1 = unpack_half2(*reinterpret_cast<const uint32_t *>(vp + WK * R::kPitch + (16 * j + r + 8) * R::kScale + 4 * gq));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const float st = y ? s1.x : s0.x, p0 = pr[j][nt][2 * y] * st, p1 = pr[j][nt][2 * y + 1] * st;
+                const uint32_t h = pack2<M>(p0, p1);
+                pb[nt][gq][y] = transpose8x8(h);
+                if (fine) {
+                  const float2 f = unpack2<M>(h);
+                  pl[nt][gq][y] = transpose8x8(pack2<M>(p0 - f.x, p1 - f.y));
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                z_run[nt][e][gq] = fmaf(pr[j][nt][e], s0.y, fmaf(pr[j][nt][e + 2], s1.y, z_run[nt][e][gq]));
+            }
+          }
+          const uint8_t *v0 = vp + (16 * j + 2 * q4) * R::kPitch;
+          if constexpr (GROUP >= 64) {
+            // word r of each 64 elements: rows m of a product are its codes i and i + 4
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+              const int at_word = 4 * (8 * h + r);
+              const uint32_t wa = *reinterpret_cast<const uint32_t *>(v0 + at_word);
+              const uint32_t wb = *reinterpret_cast<const uint32_t *>(v0 + R::kPitch + at_word);
+              const uint32_t wc = *reinterpret_cast<const uint32_t *>(v0 + 8 * R::kPitch + at_word);
+              const uint32_t wd = *reinterpret_cast<const uint32_t *>(v0 + 9 * R::kPitch + at_word);
+              uint32_t x[4] = {__byte_perm(wa, wb, 0x5410), __byte_perm(wa, wb, 0x7632), __byte_perm(wc, wd, 0x5410),
+                               __byte_perm(wc, wd, 0x7632)};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t mask = i & 1 ? 0x00F000F0u : 0x000F000Fu;
+                if (i == 2) {
+#pragma unroll
+                  for (int y = 0; y < 4; ++y) x[y] >>= 8;
+                }
+                const uint32_t a[4] = {x[0] & mask, x[1] & mask, x[2] & mask, x[3] & mask};
+                constexpr int GQ = GROUP / 64 > 0 ? GROUP / 64 : 1;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  mma<M>(o[4 * h + i][nt], a, pb[nt][h / GQ][0], pb[nt][h / GQ][1]);
+                  if (fine) mma<M>(o[4 * h + i][nt], a, pl[nt][h / GQ][0], pl[nt][h / GQ][1]);
+                }
+              }
+            }
+          } else {
+            // half-word r of each 32 elements: rows m are its codes i and i + 2
+#pragma unroll
+            for (int h = 0; h < D / 32; ++h) {
+              const int at_half = 2 * (8 * h + r);
+              const uint32_t wa = *reinterpret_cast<const uint16_t *>(v0 + at_half);
+              const uint32_t wb = *reinterpret_cast<const uint16_t *>(v0 + R::kPitch + at_half);
+              const uint32_t wc = *reinterpret_cast<const uint16_t *>(v0 + 8 * R::kPitch + at_half);
+              const uint32_t wd = *reinterpret_cast<const uint16_t *>(v0 + 9 * R::kPitch + at_half);
+              const uint32_t x = wa | (wb << 16), y = wc | (wd << 16);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t mask = i & 1 ? 0x00F000F0u : 0x000F000Fu;
+                const uint32_t a[4] = {x & mask, (x >> 8) & mask, y & mask, (y >> 8) & mask};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  mma<M>(o[2 * h + i][nt], a, pb[nt][h][0], pb[nt][h][1]);
+                  if (fine) mma<M>(o[2 * h + i][nt], a, pl[nt][h][0], pl[nt][h][1]);
+                }
+              }
+            }
+          }
+        }
+      }
+      stage = stage + 1 == R::kStages ? 0 : stage + 1;
+    }
+    cp_wait<0>();
+    __syncthreads();  // every warp is done with its ring: it becomes the join buffer
+
+    // ---- join the four warps
+    float *buf = reinterpret_cast<float *>(smem);  // [warp][kRows][D + kRowPad]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float l = l_run[nt][e];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        float z[NG];
+#pragma unroll
+        for (int gq = 0; gq < NG; ++gq) {
+          z[gq] = 0.f;
+          if (GROUP != 0) {
+            z[gq] = z_run[nt][e][gq];
+            z[gq] += __shfl_xor_sync(0xffffffffu, z[gq], 4);
+            z[gq] += __shfl_xor_sync(0xffffffffu, z[gq], 8);
+            z[gq] += __shfl_xor_sync(0xffffffffu, z[gq], 16);
+          }
+        }
+        const int row = nt * 8 + 2 * q4 + e;
+        float *to = buf + (warp * kRows + row) * (D + kRowPad);
+        if (r == 0) stat_m[warp * kRows + row] = m_run[nt][e], stat_l[warp * kRows + row] = l;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float v = o[mt][nt][e + 2 * y];
+            if constexpr (GROUP == 0) {
+              to[16 * mt + r + 8 * y] = v;
+            } else if constexpr (GROUP >= 64) {
+              constexpr int GQ = GROUP / 64 > 0 ? GROUP / 64 : 1;
+              const int h = mt / 4, i = mt % 4;
+              to[64 * h + 8 * r + i + 4 * y] = fmaf(v, i & 1 ? 0x1p20f : 0x1p24f, z[h / GQ]);
+            } else {
+              const int h = mt / 2, i = mt % 2;
+              to[32 * h + 4 * r + i + 2 * y] = fmaf(v, i & 1 ? 0x1p20f : 0x1p24f, z[h]);
+            }
+          }
+      }
+    __syncthreads();
+    const bool whole = i0 == 0 && i1 == tk.n_blocks;
+    float *part = P.partials + ((int64_t)blockIdx.x * 2 + (cur != begin)) * kRows * (D + 2);
+    for (int row = warp; row < kRows; row += kWarps) {
+      int t, h;
+      if (!row_place(row, t, h)) continue;
+      float m = -INFINITY, l = 0.f, w[kWarps];
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) m = fmaxf(m, stat_m[k * kRows + row]);
+      const float base = m > -INFINITY ? m : 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        w[k] = tc::ex2_approx(stat_m[k * kRows + row] - base);
+        l = fmaf(w[k], stat_l[k * kRows + row], l);
+      }
+      float acc[D / 32];
+      bool odd = !isfinite(l);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        acc[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k)
+          acc[i] = fmaf(w[k], buf[(k * kRows + row) * (D + kRowPad) + lane + 32 * i], acc[i]);
+        odd |= !isfinite(acc[i]);
+      }
+      // rows of a tile of one token see the same keys: nothing unseen was multiplied
+      if (ntok > 1 && __any_sync(0xffffffffu, odd)) {
+        const char *qp = reinterpret_cast<const char *>(A.q.data) + 2 * ((int64_t)t * A.q.stride_token + (int64_t)h * A.q.stride_head);
+        float *to = buf + row * (D + kRowPad);  // read above, not needed any more
+        __syncwarp();
+        redo_row<D, GROUP>(P, tk, b, g, i0, i1, load_position(A.batch, t), qp, to, &stat_m[row], &stat_l[row]);
+        __syncwarp();
+        m = stat_m[row], l = stat_l[row];
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[i] = to[lane + 32 * i];
+      }
+      if (whole) {
+        // l is 0 only if no key is seen (a NaN score makes it NaN)
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+          store_any(A.out.data, (int64_t)t * A.out.stride_token + (int64_t)h * A.out.stride_head + lane + 32 * i,
+                    acc[i] * inv, P.dtype);
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) part[row * D + lane + 32 * i] = acc[i];
+        if (lane == 0) part[kRows * D + row] = m, part[kRows * D + kRows + row] = l;
+      }
+    }
+    cur += i1 - i0;
+    __syncthreads();  // the join buffer becomes the ring again
+  }
+}
+
+// Joins the pieces of each tile that a border cut: CTA k takes the tile that
+// k's range starts in if k is the first to start inside it; the pieces lie in
+// the second slot of CTA k - 1 (its first, if its range starts with the tile)
+// and the first slots of k, k + 1, ...
+template <int D>
+__global__ void __launch_bounds__(256) join_kernel(const DecodeParams P, int rows) {
+  const int k = blockIdx.x;
+  const CutUnit c = P.cuts[k];
+  if (k == 0 || k >= c.n_ctas) return;
+  const int64_t mine = cut_at(c.total, c.n_ctas, k), before = cut_at(c.total, c.n_ctas, k - 1);
+  if (mine == c.start || before > c.start) return;
+  int last = k;
+  while (last + 1 < c.n_ctas && cut_at(c.total, c.n_ctas, last + 1) < c.end) ++last;
+  const int lane = threadIdx.x % 32;
+  const int64_t slot = (int64_t)rows * (D + 2);
+  const float *first = P.partials + ((int64_t)(k - 1) * 2 + (before != c.start)) * slot;
+  for (int row = threadIdx.x / 32; row < rows; row += blockDim.x / 32) {
+    const int pi = row / P.heads_per_tile, hh = row - pi * P.heads_per_tile;
+    if (pi >= c.n_tok || hh >= c.n_heads) continue;
+    float m = -INFINITY;
+    for (int j = k - 1 + lane; j <= last; j += 32)
+      m = fmaxf(m, (j < k ? first : P.partials + (int64_t)j * 2 * slot)[rows * D + row]);
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float base = m > -INFINITY ? m : 0.f;
+    float l = 0.f, acc[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+#pragma unroll 4
+    for (int j = k - 1; j <= last; ++j) {
+      const float *part = j < k ? first : P.partials + (int64_t)j * 2 * slot;
+      const float w = tc::ex2_approx(part[rows * D + row] - base);
+      l = fmaf(w, part[rows * D + rows + row], l);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(w, part[row * D + lane + 32 * i], acc[i]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t at = (int64_t)(c.tok + pi) * P.a.out.stride_token + (int64_t)(c.head + hh) * P.a.out.stride_head;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) store_any(P.a.out.data, at + lane + 32 * i, acc[i] * inv, P.dtype);
+  }
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return n > 0 ? n : 148;
+}
+
+// Rows of a tile: eight where a request's rows fit them, else sixteen.
+int tile_rows(const AttendParams &P) {
+  const int64_t per_request = ((int64_t)P.batch.n_tokens + P.batch.batch - 1) / P.batch.batch;
+  return P.G * per_request <= 8 ? 8 : 16;
+}
+
+int max_grid(const AttendParams &P, int resident) {
+  // no more CTAs than blocks there can be
+  const int64_t tiles = (int64_t)P.batch.n_tokens * P.Hq;
+  const int64_t blocks = ((int64_t)P.batch.max_blocks * P.cache.block_size + 63) / 64 + 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)resident * sm_count(), tiles * blocks));
+}
+constexpr int kMaxResident = 4;
+
+template <typename T, int D, int GROUP, int NT>
+int run(const DecodeParams &P, cudaStream_t st) {
+  auto kernel = decode_kernel<T, D, GROUP, NT>;
+  constexpr int kSmem = smem_bytes<D, GROUP, NT>();
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+  if (ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), kSmem) != SB_OK) return SB_ERR_CUDA;
+  constexpr int kResident = std::min(kMaxResident, (227 * 1024) / (kSmem + 1024));
+  const int grid = max_grid(P.a, kResident);
+  const int slot = prof_before(st);
+  kernel<<<grid, kThreads, kSmem, st>>>(P);
+  prof_after(slot, st);
+  int s = launch_status();
+  if (s != SB_OK || grid == 1) return s;
+  join_kernel<D><<<grid, 256, 0, st>>>(P, 8 * NT);
+  return launch_status();
+}
+
+template <typename T, int D, int GROUP>
+int by_rows(const DecodeParams &P, int rows, cudaStream_t st) {
+  return rows == 8 ? run<T, D, GROUP, 1>(P, st) : run<T, D, GROUP, 2>(P, st);
+}
+
+}  // namespace
+
+// 16-bit rows or codes of head_dim 64 or 128 whose rows and queries start at multiples of 16 bytes.
+bool decode_takes(const AttendParams &P, int dtype) {
+  if (dtype == SB_DTYPE_F32 || (P.cache.head_dim != 64 && P.cache.head_dim != 128)) return false;
+  if (!rows_aligned(P.q, 2, 16)) return false;
+  if (P.cache.group == 0) return cache_aligned(P.cache, 2, 16);
+  const int sb = 4 * (P.cache.head_dim / P.cache.group);  // a row's scales are copied in one piece
+  return multiple(P.cache.scales, sb) && multiple(P.cache.scale_block * 2, sb) && multiple(P.cache.scale_kv * 2, sb) &&
+         multiple(P.cache.scale_head * 2, sb) && multiple(P.cache.scale_pos * 2, sb);
+}
+
+int64_t decode_workspace_bytes(const AttendParams &P) {
+  const int64_t grid = max_grid(P, kMaxResident);
+  return ((grid * (int64_t)sizeof(CutUnit) + 15) / 16) * 16 + grid * 2 * 16 * (P.cache.head_dim + 2) * 4;
+}
+
+int launch_decode(const AttendParams &A, int dtype, void *workspace, cudaStream_t st) {
+  DecodeParams P;
+  P.dtype = dtype;
+  const int rows = tile_rows(A);
+  const int64_t cut_bytes = ((int64_t)max_grid(A, kMaxResident) * (int64_t)sizeof(CutUnit) + 15) / 16 * 16;
+  P.cuts = reinterpret_cast<CutUnit *>(workspace);
+  P.partials = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + cut_bytes);
+  P.heads_per_tile = std::min(A.G, rows);
+  P.tokens_per_tile = rows / P.heads_per_tile;
+  P.head_tiles = (A.G + P.heads_per_tile - 1) / P.heads_per_tile;
+  // a launch takes at most kMaxRequests requests; later ones of the stream reuse the workspace
+  for (int b = 0; b < A.batch.batch; b += kMaxRequests) {
+    P.a = A;
+    P.a.batch.batch = std::min(kMaxRequests, A.batch.batch - b);
+    P.a.batch.cu_seqlens += b;
+    P.a.batch.block_tables = reinterpret_cast<const char *>(A.batch.block_tables) +
+                             (int64_t)b * A.batch.table_stride * (A.batch.table_dtype == SB_INDEX_I64 ? 8 : 4);
+    int s;
+    const int D = A.cache.head_dim;
+    switch (A.cache.group) {
+      case 0:
+        if (dtype == SB_DTYPE_BF16)
+          s = D == 128 ? by_rows<__nv_bfloat16, 128, 0>(P, rows, st) : by_rows<__nv_bfloat16, 64, 0>(P, rows, st);
+        else
+          s = D == 128 ? by_rows<__half, 128, 0>(P, rows, st) : by_rows<__half, 64, 0>(P, rows, st);
+        break;
+      case 32: s = D == 128 ? by_rows<__half, 128, 32>(P, rows, st) : by_rows<__half, 64, 32>(P, rows, st); break;
+      case 64: s = D == 128 ? by_rows<__half, 128, 64>(P, rows, st) : by_rows<__half, 64, 64>(P, rows, st); break;
+      default: s = by_rows<__half, 128, 128>(P, rows, st);
+    }
+    if (s != SB_OK) return s;
+  }
+  return SB_OK;
+}
+
+}  // namespace paged
+}  // namespace sb

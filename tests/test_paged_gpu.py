@@ -9,8 +9,10 @@ Tolerances count roundings (u = half a step of a type, relative):
 * 4-bit rows: none; codes, steps and zeros are functions of the fp32 values,
   which the 64-bit rotation pins;
 * attention: one rounding of the result, u * |out|; one rounding of each
-  probability to the type the products take, u_p * sum_j w_j |v_j|; the fp32
-  sums, and the scores: a sum of D products in steps of 16 loses at most
+  probability to the type the products take, u_p * sum_j w_j |v_j|, or, over a
+  4-bit cache and a bf16 result, of each probability times its key's step to
+  fp16, which multiplies the code alone (the zero's part is summed in fp32):
+  2^-11 * sum_j w_j step_j code_j; the fp32 sums, and the scores: a sum of D products in steps of 16 loses at most
   2^-23 per step of the largest partial sum, and moves the result by twice that
   times sum_j w_j |v_j|.
 """
@@ -111,6 +113,10 @@ def check_attention(c: Case, got, *, window=None, sinks=0, scale=None):
     partial = reach * (1.0 if c.group is None else 1039.0 / 7.5)
     delta = (c.d / 16 + 2) * 2.0**-23 * partial + 2.0**-21
     tol = u * want.abs() + (u + 2.0**-20 + 2 * delta[..., None]) * spread + 2.0**-25
+    if c.group is not None and c.dtype == BF:
+        coded = c.value_cache()
+        coded[:, 1] -= c.scales[:, 1, ..., 1].double().repeat_interleave(c.group, -1)  # step * code
+        tol += 2.0**-11 * op.attention(c.q, coded, c.tables, c.cu, c.positions, window, sinks, scale)[0]
     if c.dtype == FP:  # a plain chain of D products
         tol = u * want.abs() + (2.0**-19 + 2 * (c.d * 2.0**-24 * partial[..., None])) * spread + 2.0**-30
     bad = ~((got[:n] - want[:n]).abs() <= tol[:n])
