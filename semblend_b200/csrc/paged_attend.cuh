@@ -77,10 +77,92 @@ __host__ __device__ __forceinline__ void request_tokens(const sb_paged_batch &B,
   if (hi < lo) hi = lo;
 }
 
+__device__ __forceinline__ float load_any(const void *p, int64_t i, int dtype) {
+  if (dtype == SB_DTYPE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]);
+  return __half2float(reinterpret_cast<const __half *>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void *p, int64_t i, float x, int dtype) {
+  if (dtype == SB_DTYPE_BF16) reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
+  else reinterpret_cast<__half *>(p)[i] = __float2half_rn(x);
+}
+
+// Address of the row of `key` in request b's pages, or false if it has none.
+__device__ __forceinline__ bool key_row(const AttendParams &P, int b, int key, int64_t &row, int64_t &scale_row) {
+  const int bs = P.cache.block_size, lb = key / bs;
+  const int phys = find_block(P.batch, b, lb, P.cache.n_blocks);
+  if (phys < 0) return false;
+  const int64_t in = key - lb * bs;
+  row = phys * P.cache.stride_block + in * P.cache.stride_pos;
+  scale_row = phys * P.cache.scale_block + in * P.cache.scale_pos;
+  return true;
+}
+
+// One element of a row of a 16-bit or 4-bit cache (K rows; V rows lie stride_kv behind).
+__device__ __forceinline__ float row_elem(const AttendParams &P, int64_t row, int64_t scale_row, int d, int dtype) {
+  if (P.cache.group == 0) return load_any(P.cache.data, row + d, dtype);
+  const uint8_t c = reinterpret_cast<const uint8_t *>(P.cache.data)[row + d / 2];
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(
+      reinterpret_cast<const __half *>(P.cache.scales) + scale_row + 2 * (d / P.cache.group)));
+  return fmaf((float)(d & 1 ? c >> 4 : c & 15), f.x, f.y);
+}
+
+// One query row over keys [k0, k1) that a token at position p sees, by one
+// warp: running maximum m (log2 units), sum l and, per lane, elements lane,
+// lane + 32, ... of the weighted sum.  For the rare rows whose tile gave an
+// infinity or a NaN that may come from a key the row does not see (a product of
+// a probability of zero); not fast.
+template <int D> struct RowSums {
+  float m, l, acc[D / 32];
+};
+template <int D>
+__device__ __noinline__ void add_keys(const AttendParams &A, int dtype, int b, int g, int p, const void *q, int k0,
+                                      int k1, RowSums<D> &r) {
+  const int lane = threadIdx.x % 32;
+  const Span sp = key_span(A, p);
+  const float c = A.scale * 1.4426950408889634f;
+  float qv[D / 32];
+  for (int i = 0; i < D / 32; ++i) qv[i] = load_any(q, lane + 32 * i, dtype);
+  for (int key = k0; key < k1; ++key) {
+    int64_t row, srow;
+    if (p < 0 || !in_span(sp, key) || !key_row(A, b, key, row, srow)) continue;
+    row += (int64_t)g * A.cache.stride_head, srow += (int64_t)g * A.cache.scale_head;
+    float dot = 0.f;
+    for (int j = 0; j < D / 32; ++j) dot = fmaf(qv[j], row_elem(A, row, srow, lane + 32 * j, dtype), dot);
+    for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
+    const float x = dot * c, m_new = fmaxf(r.m, x), base = m_new > -INFINITY ? m_new : 0.f;
+    const float corr = r.m > -INFINITY ? exp2f(r.m - base) : 0.f, w = exp2f(x - base);
+    r.m = m_new, r.l = r.l * corr + w;
+    for (int j = 0; j < D / 32; ++j)
+      r.acc[j] = fmaf(w, row_elem(A, row + A.cache.stride_kv, srow + A.cache.scale_kv, lane + 32 * j, dtype),
+                      r.acc[j] * corr);
+  }
+}
+template <int D> __device__ __forceinline__ void clear(RowSums<D> &r) {
+  r.m = -INFINITY, r.l = 0.f;
+  for (int i = 0; i < D / 32; ++i) r.acc[i] = 0.f;
+}
+// The whole row, written to o.
+template <int D>
+__device__ __noinline__ void attend_row(const AttendParams &A, int dtype, int b, int g, int p, const void *q, void *o) {
+  RowSums<D> r;
+  clear(r);
+  const Span sp = key_span(A, p);
+  add_keys<D>(A, dtype, b, g, p, q, 0, sp.sink_end, r);
+  add_keys<D>(A, dtype, b, g, p, q, sp.first, sp.end, r);
+  const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
+  for (int i = 0; i < D / 32; ++i) store_any(o, threadIdx.x % 32 + 32 * i, r.acc[i] * inv, dtype);
+}
+
 // Decode path (csrc/paged_decode.cu): tiles of 8 or 16 query rows, keys split over CTAs.
 bool decode_takes(const AttendParams &P, int dtype);
 int64_t decode_workspace_bytes(const AttendParams &P);
 int launch_decode(const AttendParams &P, int dtype, void *workspace, cudaStream_t st);
+
+
+// Prefill path (csrc/paged_prefill.cu): tiles of 128 query rows on tcgen05.
+constexpr int kPrefillWorkspace = 16;
+bool prefill_takes(const AttendParams &P, int dtype);
+int launch_prefill(const AttendParams &P, int dtype, int32_t *status, void *workspace, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace sb

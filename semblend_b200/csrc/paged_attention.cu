@@ -121,7 +121,8 @@ extern "C" SB_API int64_t sb_paged_attention_workspace_bytes(const sb_paged_cach
   paged::AttendParams P = {};
   P.cache = *cache, P.batch = *batch;
   P.Hq = n_q_heads, P.G = n_q_heads / cache->n_heads;
-  return paged::decode_takes(P, dtype) ? paged::decode_workspace_bytes(P) : 0;
+  P.scale = 1.f;
+  return paged::decode_takes(P, dtype) ? std::max<int64_t>(paged::decode_workspace_bytes(P), paged::kPrefillWorkspace) : 0;
 }
 
 extern "C" SB_API int sb_paged_attention(const sb_paged_cache *cache, const sb_paged_batch *batch,
@@ -149,6 +150,10 @@ extern "C" SB_API int sb_paged_attention(const sb_paged_cache *cache, const sb_p
   P.sinks = window ? sinks : 0;
   P.scale = scale;
   if (paged::decode_takes(P, dtype)) {
+    const bool prefill = paged::prefill_takes(P, dtype);
+    if (!workspace || workspace_bytes < paged::kPrefillWorkspace || !paged::multiple(workspace, 16))
+      return SB_ERR_WORKSPACE_TOO_SMALL;
+    if (prefill) return paged::launch_prefill(P, dtype, status, workspace, st);
     if (!workspace || workspace_bytes < paged::decode_workspace_bytes(P) || !paged::multiple(workspace, 16))
       return SB_ERR_WORKSPACE_TOO_SMALL;
     return paged::launch_decode(P, dtype, workspace, st);

@@ -138,71 +138,6 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x) {
   return std::is_same<T, __nv_bfloat16>::value ? unpack_bf2(x) : unpack_half2(x);
 }
 
-__device__ __forceinline__ float load_any(const void *p, int64_t i, int dtype) {
-  if (dtype == SB_DTYPE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]);
-  return __half2float(reinterpret_cast<const __half *>(p)[i]);
-}
-__device__ __forceinline__ void store_any(void *p, int64_t i, float x, int dtype) {
-  if (dtype == SB_DTYPE_BF16) reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
-  else reinterpret_cast<__half *>(p)[i] = __float2half_rn(x);
-}
-
-// Address of the row of `key` in request b's pages, or false if it has none.
-__device__ __forceinline__ bool key_row(const AttendParams &P, int b, int key, int64_t &row, int64_t &scale_row) {
-  const int bs = P.cache.block_size, lb = key / bs;
-  const int phys = find_block(P.batch, b, lb, P.cache.n_blocks);
-  if (phys < 0) return false;
-  const int64_t in = key - lb * bs;
-  row = phys * P.cache.stride_block + in * P.cache.stride_pos;
-  scale_row = phys * P.cache.scale_block + in * P.cache.scale_pos;
-  return true;
-}
-
-// One element of a row of the cache (K rows; V rows lie stride_kv behind).
-template <int GROUP>
-__device__ __forceinline__ float row_elem(const AttendParams &P, int64_t row, int64_t scale_row, int d, int dtype) {
-  if (GROUP == 0) return load_any(P.cache.data, row + d, dtype);
-  const uint8_t c = reinterpret_cast<const uint8_t *>(P.cache.data)[row + d / 2];
-  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(
-      reinterpret_cast<const __half *>(P.cache.scales) + scale_row + 2 * (d / (GROUP == 0 ? 1 : GROUP))));
-  return fmaf((float)(d & 1 ? c >> 4 : c & 15), f.x, f.y);
-}
-
-// The rows of a tile whose sums came out infinite or NaN although a product
-// with a probability of zero may be why (a key another row of the tile sees
-// holds an infinity or a NaN): the same sums over keys [from blocks i0 to i1)
-// that this row sees, one warp a row.  Rare, and not fast.
-template <int D, int GROUP>
-__device__ __noinline__ void redo_row(const DecodeParams &P, const TileKeys &tk, int b, int g, int i0, int i1, int p,
-                                      const void *q, float *o, float *m_out, float *l_out) {
-  constexpr int KB = Ring<D, GROUP>::kBlock;
-  const AttendParams &A = P.a;
-  const int lane = threadIdx.x % 32;
-  const Span sp = key_span(A, p);
-  constexpr int kPer = D / 32;
-  float qv[kPer], acc[kPer], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < kPer; ++i) qv[i] = load_any(q, lane + 32 * i, P.dtype), acc[i] = 0.f;
-  const float c = A.scale * 1.4426950408889634f;
-  for (int i = i0; i < i1; ++i)
-    for (int k = 0; k < KB; ++k) {
-      const int key = block_key(tk, i, KB) + k;
-      int64_t row, srow;
-      if (p < 0 || !in_span(sp, key) || !key_row(A, b, key, row, srow)) continue;
-      row += (int64_t)g * A.cache.stride_head, srow += (int64_t)g * A.cache.scale_head;
-      float dot = 0.f;
-      for (int j = 0; j < kPer; ++j) dot = fmaf(qv[j], row_elem<GROUP>(A, row, srow, lane + 32 * j, P.dtype), dot);
-      for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-      const float x = dot * c, m_new = fmaxf(m, x), base = m_new > -INFINITY ? m_new : 0.f;
-      const float corr = m > -INFINITY ? exp2f(m - base) : 0.f, w = exp2f(x - base);
-      m = m_new, l = l * corr + w;
-      for (int j = 0; j < kPer; ++j)
-        acc[j] = fmaf(w, row_elem<GROUP>(A, row + A.cache.stride_kv, srow + A.cache.scale_kv, lane + 32 * j, P.dtype),
-                      acc[j] * corr);
-    }
-  for (int i = 0; i < kPer; ++i) o[lane + 32 * i] = acc[i];
-  if (lane == 0) *m_out = m, *l_out = l;
-}
-
 template <typename T, int D, int GROUP, int NT>
 __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) {
   using R = Ring<D, GROUP>;
@@ -774,13 +709,15 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) 
       // rows of a tile of one token see the same keys: nothing unseen was multiplied
       if (ntok > 1 && __any_sync(0xffffffffu, odd)) {
         const char *qp = reinterpret_cast<const char *>(A.q.data) + 2 * ((int64_t)t * A.q.stride_token + (int64_t)h * A.q.stride_head);
-        float *to = buf + row * (D + kRowPad);  // read above, not needed any more
-        __syncwarp();
-        redo_row<D, GROUP>(P, tk, b, g, i0, i1, load_position(A.batch, t), qp, to, &stat_m[row], &stat_l[row]);
-        __syncwarp();
-        m = stat_m[row], l = stat_l[row];
+        RowSums<D> sums;
+        clear(sums);
+        for (int i = i0; i < i1; ++i) {
+          const int key0 = block_key(tk, i, KB);
+          add_keys<D>(A, P.dtype, b, g, load_position(A.batch, t), qp, key0, key0 + KB, sums);
+        }
+        m = sums.m, l = sums.l;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[i] = to[lane + 32 * i];
+        for (int i = 0; i < D / 32; ++i) acc[i] = sums.acc[i];
       }
       if (whole) {
         // l is 0 only if no key is seen (a NaN score makes it NaN)
