@@ -439,7 +439,76 @@ __global__ void __launch_bounds__(Shape<D, CODES>::kThreads, 1)
             row = row1, blk = blk1;
           }
         } else {
-          // CODES_LOADER
+          // Rows of kLanes threads, 32 codes (16 bytes) each; this warp takes groups of rows
+          // loader, loader + 7, ... of a block.  The next block's codes are on their way to registers
+          // while this one waits for its slot.
+          constexpr int kLanes = D / 32, kRows = 32 / kLanes, kGroups = kBN / kRows;
+          constexpr int kMine = (kGroups + S::kLoaders - 1) / S::kLoaders;
+          const int loader = leader ? 0 : warp - 9, chunk = lane % kLanes;
+          const char *cbase = reinterpret_cast<const char *>(A.cache.data) + (int64_t)w.g * A.cache.stride_head + 16 * chunk;
+          const char *sbase = reinterpret_cast<const char *>(A.cache.scales) + 2 * (int64_t)w.g * A.cache.scale_head +
+                              4 * (32 * chunk / A.cache.group);
+          uint4 code[2][kMine];
+          uint32_t scale[2][kMine];  // (step, zero); both 0 where no row of the unit sees the key
+          auto fetch = [&](int i, int kv) {
+#pragma unroll
+            for (int x = 0; x < kMine; ++x) {
+              const int key = unit_block_key(w, i) + (loader + x * S::kLoaders) * kRows + lane / kLanes;
+              code[kv][x] = make_uint4(0, 0, 0, 0);
+              scale[kv][x] = 0u;
+              int64_t row, srow;
+              if (loader + x * S::kLoaders < kGroups && key < w.end && (key >= w.first || key < w.sink_end) &&
+                  key_row(A, w.b, key, row, srow)) {
+                code[kv][x] = *reinterpret_cast<const uint4 *>(cbase + row + kv * A.cache.stride_kv);
+                scale[kv][x] = *reinterpret_cast<const uint32_t *>(sbase + 2 * (srow + kv * A.cache.scale_kv));
+              }
+            }
+          };
+          auto store = [&](uint8_t *tile, int kv) {
+#pragma unroll
+            for (int x = 0; x < kMine; ++x) {
+              if (loader + x * S::kLoaders >= kGroups) continue;
+              const int row = (loader + x * S::kLoaders) * kRows + lane / kLanes;
+              const __half2 sz = *reinterpret_cast<const __half2 *>(&scale[kv][x]);
+              const __half2 step = __low2half2(sz), zero = __high2half2(sz);
+              const uint32_t word[4] = {code[kv][x].x, code[kv][x].y, code[kv][x].z, code[kv][x].w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                // 0x6400 | c is 1024 + c in fp16, 0x6400 | 16 c is 1024 + 16 c; both back to c exactly
+                uint32_t out[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  const uint32_t b = (((y < 2 ? word[i] : word[i] >> 8) & (y & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u);
+                  const __half2 raw = *reinterpret_cast<const __half2 *>(&b);
+                  const __half2 c = y & 1 ? __hfma2(raw, __float2half2_rn(0.0625f), __float2half2_rn(-64.f))
+                                          : __hsub2(raw, __float2half2_rn(1024.f));
+                  const __half2 v = __hfma2(c, step, zero);
+                  out[y] = *reinterpret_cast<const uint32_t *>(&v);
+                }
+                const int at = 4 * chunk + i;  // eight elements: one 16-byte piece of the row
+                *reinterpret_cast<uint4 *>(tile + (at / 8) * kHalf + row * 128 + (((at % 8) ^ (row & 7)) << 4)) =
+                    make_uint4(out[0], out[1], out[2], out[3]);
+              }
+            }
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+          };
+          fetch(0, 0);
+          fetch(0, 1);
+          for (int j = 0; j < nb && ok; ++j) {
+            const uint32_t st = gl % kStages, ph = (gl / kStages) & 1;
+            ok = __all_sync(0xffffffffu, tc::mbar_wait(&k_empty[st], ph ^ 1, ab, 2, kWaitCycles));
+            if (!ok) break;
+            store(sK + st * kTile, 0);
+            if (lane == 0) tc::mbar_arrive(&k_full[st]);
+            if (j + 1 < nb) fetch(j + 1, 0);
+            ok = __all_sync(0xffffffffu, tc::mbar_wait(&v_empty[st], ph ^ 1, ab, 2, kWaitCycles));
+            if (!ok) break;
+            store(sV + st * kTile, 1);
+            if (lane == 0) tc::mbar_arrive(&v_full[st]);
+            if (j + 1 < nb) fetch(j + 1, 1);
+            ++gl;
+          }
         }
       }
       if (!CODES && lane == 0) {
@@ -762,7 +831,6 @@ bool prefill_takes(const AttendParams &P, int dtype) {
   if (bs % 8 || (bs < kBN ? kBN % bs : bs % kBN)) return false;
   const PrefillParams p = plan(P);
   if (p.n_units >= (1ll << 31)) return false;
-  if (P.cache.group != 0) return false;  // CODES_RULE
   return (int64_t)P.batch.n_tokens * P.G >= 64 * (int64_t)P.batch.batch;
 }
 
@@ -770,7 +838,8 @@ int launch_prefill(const AttendParams &A, int dtype, int32_t *status, void *work
   PrefillParams P = plan(A);
   P.dtype = dtype;
   const bool wide = A.cache.head_dim == 128;
-  // CODES_LAUNCH
+  if (A.cache.group != 0)
+    return wide ? run<__half, 128, true>(P, status, workspace, st) : run<__half, 64, true>(P, status, workspace, st);
   if (dtype == SB_DTYPE_BF16)
     return wide ? run<__nv_bfloat16, 128, false>(P, status, workspace, st)
                 : run<__nv_bfloat16, 64, false>(P, status, workspace, st);
