@@ -141,18 +141,6 @@ template <int D> __device__ __forceinline__ void clear(RowSums<D> &r) {
   r.m = -INFINITY, r.l = 0.f;
   for (int i = 0; i < D / 32; ++i) r.acc[i] = 0.f;
 }
-// The whole row, written to o.
-template <int D>
-__device__ __noinline__ void attend_row(const AttendParams &A, int dtype, int b, int g, int p, const void *q, void *o) {
-  RowSums<D> r;
-  clear(r);
-  const Span sp = key_span(A, p);
-  add_keys<D>(A, dtype, b, g, p, q, 0, sp.sink_end, r);
-  add_keys<D>(A, dtype, b, g, p, q, sp.first, sp.end, r);
-  const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
-  for (int i = 0; i < D / 32; ++i) store_any(o, threadIdx.x % 32 + 32 * i, r.acc[i] * inv, dtype);
-}
-
 // Decode path (csrc/paged_decode.cu): tiles of 8 or 16 query rows, keys split over CTAs.
 bool decode_takes(const AttendParams &P, int dtype);
 int64_t decode_workspace_bytes(const AttendParams &P);
@@ -160,7 +148,8 @@ int launch_decode(const AttendParams &P, int dtype, void *workspace, cudaStream_
 
 
 // Prefill path (csrc/paged_prefill.cu): tiles of 128 query rows on tcgen05.
-constexpr int kPrefillWorkspace = 16;
+constexpr int kPrefillWorkspace = 128;  // unit counter and status, ahead of expanded rows
+int64_t prefill_workspace_bytes(const AttendParams &P);
 bool prefill_takes(const AttendParams &P, int dtype);
 int launch_prefill(const AttendParams &P, int dtype, int32_t *status, void *workspace, cudaStream_t st);
 
