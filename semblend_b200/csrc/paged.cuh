@@ -2,6 +2,8 @@
 // the argument checks of their C entry points.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace sb {
@@ -39,6 +41,19 @@ __host__ __device__ __forceinline__ int find_block(const sb_paged_batch &B, int 
 __host__ __device__ __forceinline__ int load_position(const sb_paged_batch &B, int t) {
   const int64_t p = index_at(B.positions, t, B.pos_dtype);
   return p < 0 ? -1 : p > 0x7fffff00 ? 0x7fffff00 : (int)p;
+}
+
+// SMs of the current device, looked up once per device.
+inline int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 inline bool index_ok(int dtype) { return dtype == SB_INDEX_I32 || dtype == SB_INDEX_I64; }

@@ -380,16 +380,9 @@ __global__ void __launch_bounds__(kThreads) gather4_kernel(const GatherParams P,
   }
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-  return n > 0 ? n : 148;
-}
-
 // Tokens a CTA takes: one while that leaves SMs without work, else four (the angles of four
 // tokens of head_dim 128 are one per thread).
-int tokens_per_cta(int n_tokens) { return n_tokens >= 4 * kMaxTokens * sm_count() ? kMaxTokens : 1; }
+int tokens_per_cta(int n_tokens) { return n_tokens >= 4 * kMaxTokens * paged::sm_count() ? kMaxTokens : 1; }
 
 template <typename T, int VEC>
 void launch_append(const AppendParams &P, bool neox, int grid, cudaStream_t st) {

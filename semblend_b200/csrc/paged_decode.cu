@@ -33,13 +33,13 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxRequests = 1024;  // of one launch: their prefix sums lie in shared memory
+constexpr int kMaxRequests = 512;  // of one launch: their prefix sums lie in shared memory
 
 // Keys a warp takes at a time, stages of its ring and bytes of one stage.
 template <int D, int GROUP> struct Ring {
   static constexpr int kKeys = GROUP == 0 ? 16 : 32;
   static constexpr int kBlock = kKeys * kWarps;
-  static constexpr int kStages = GROUP == 0 ? (D == 128 ? 3 : 5) : 4;
+  static constexpr int kStages = GROUP == 0 ? (D == 128 ? 3 : 5) : 3;
   static constexpr int kRow = GROUP == 0 ? D * 2 : D / 2;  // bytes of a row
   // code rows are 16 bytes apart beyond their length: eight rows then start in different banks
   static constexpr int kPitch = GROUP == 0 ? kRow : kRow + 16;
@@ -49,6 +49,7 @@ template <int D, int GROUP> struct Ring {
   static constexpr int kWarp = kStages * kStage;
 };
 
+constexpr int kWholeKeys = 1024;  // contexts up to this are not split
 constexpr int kRowPad = 4;  // floats between rows of the join buffer
 template <int D, int GROUP, int NT> constexpr int ring_bytes() {
   return std::max(kWarps * Ring<D, GROUP>::kWarp, kWarps * 8 * NT * (D + kRowPad) * 4);
@@ -57,11 +58,18 @@ template <int D, int GROUP, int NT> constexpr int smem_bytes() {
   return ring_bytes<D, GROUP, NT>() + (kMaxRequests + 1) * 8 + kWarps * 8 * 4 + kWarps * 8 * NT * 8 + 64;
 }
 
+// CTAs of an SM: what shared memory holds, and no more than leaves a thread the registers it needs (the
+// accumulators of sixteen rows of 128 take 64 of them).
+constexpr int kMaxResident = 4;
+template <int D, int GROUP, int NT> constexpr int resident() {
+  return std::min({kMaxResident, (227 * 1024) / (smem_bytes<D, GROUP, NT>() + 1024), D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3)});
+}
+
 // What CTA k leaves for the kernel that joins: the unit its range starts in.
 struct CutUnit {
   int64_t start, end;  // blocks of the unit in the call's line of blocks
-  int64_t total;
-  int n_ctas;
+  int64_t base;        // every CTA's blocks, and the `more` first ones take one more
+  int more, n_ctas;
   int tok, n_tok, head, n_heads;  // head: first query head of the tile
   int pad;
 };
@@ -71,15 +79,24 @@ struct DecodeParams {
   CutUnit *cuts;    // [grid]
   float *partials;  // [grid][2][R * (D + 2)]
   int tokens_per_tile, heads_per_tile, head_tiles;
+  int page_shift;   // block_size as a power of two, or -1
+  int whole;        // 1: tiles are not cut, the line counts them instead of their blocks
   int dtype;
 };
 
-// First block of CTA k.
-__host__ __device__ __forceinline__ int64_t cut_at(int64_t total, int n_ctas, int k) {
-  return total / n_ctas * k + total % n_ctas * k / n_ctas;
+// First block of CTA k, and the CTA that block x belongs to.
+__host__ __device__ __forceinline__ int64_t cut_at(int64_t base, int more, int k) {
+  return base * k + (k < more ? k : more);
+}
+__host__ __device__ __forceinline__ int cta_of(int64_t base, int more, int64_t x) {
+  const int64_t big = (base + 1) * more;
+  return (int)(x < big ? x / (base + 1) : more + (x - big) / base);
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool take) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool take) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
 template <int N> __device__ __forceinline__ void cp_async_small(uint32_t dst, const void *src, bool take) {
@@ -139,7 +156,7 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x) {
 }
 
 template <typename T, int D, int GROUP, int NT>
-__global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) {
+__global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_kernel(const DecodeParams P) {
   using R = Ring<D, GROUP>;
   // products of codes run in fp16, which holds them exactly; rows in their own type
   using M = typename std::conditional<GROUP == 0, T, __half>::type;
@@ -162,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) 
     request_tokens(A.batch, b, lo, hi);
     int64_t n = 0;
     for (int t = lo; t < hi; t += P.tokens_per_tile)
-      n += tile_keys(A, t, min(P.tokens_per_tile, hi - t), KB).n_blocks;
+      n += P.whole ? 1 : tile_keys(A, t, min(P.tokens_per_tile, hi - t), KB).n_blocks;
     prefix[b + 1] = n * P.head_tiles * Hkv;
   }
   __syncthreads();
@@ -182,13 +199,16 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) 
   __syncthreads();
   const int64_t total = prefix[B];
   const int n_ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, total));
-  int64_t cur = cut_at(total, n_ctas, blockIdx.x);
-  const int64_t stop = (int)blockIdx.x < n_ctas ? cut_at(total, n_ctas, blockIdx.x + 1) : cur;
+  const int64_t base_blocks = total / n_ctas;
+  const int more = (int)(total - base_blocks * n_ctas);
+  int64_t cur = cut_at(base_blocks, more, blockIdx.x);
+  const int64_t stop = (int)blockIdx.x < n_ctas ? cut_at(base_blocks, more, blockIdx.x + 1) : cur;
   const int64_t begin = cur;
   if (cur >= stop) {
-    if (tid == 0) P.cuts[blockIdx.x].n_ctas = 0;
+    if (tid == 0 && !P.whole) P.cuts[blockIdx.x].n_ctas = 0;
     return;
   }
+  const bool wide_table = A.batch.table_dtype == SB_INDEX_I64;
 
   const uint32_t ring = tc::smem_u32(smem) + warp * R::kWarp;
   const uint8_t *ring_ptr = smem + warp * R::kWarp;
@@ -216,22 +236,22 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) 
     for (;;) {
       ntok = min(P.tokens_per_tile, thi - tok);
       tk = tile_keys(A, tok, ntok, KB);
-      const int64_t span = (int64_t)tk.n_blocks * P.head_tiles;
+      const int weight = P.whole ? 1 : tk.n_blocks;
+      const int64_t span = (int64_t)weight * P.head_tiles;
       if (cur < at + span) {
-        ht = (int)((cur - at) / tk.n_blocks);
-        at += (int64_t)ht * tk.n_blocks;
+        if (P.head_tiles > 1) ht = (int)((cur - at) / weight), at += (int64_t)ht * weight;
         break;
       }
       at += span;
       tok += P.tokens_per_tile;
     }
-    const int i0 = (int)(cur - at);
-    const int i1 = (int)min((int64_t)tk.n_blocks, i0 + (stop - cur));
+    const int i0 = P.whole ? 0 : (int)(cur - at);
+    const int i1 = P.whole ? tk.n_blocks : (int)min((int64_t)tk.n_blocks, i0 + (stop - cur));
     const int head0 = g * A.G + ht * P.heads_per_tile;
     const int nheads = min(P.heads_per_tile, A.G - ht * P.heads_per_tile);
-    if (cur == begin && tid == 0) {
+    if (cur == begin && tid == 0 && !P.whole) {  // whole tiles leave nothing to join
       CutUnit c;
-      c.start = at, c.end = at + tk.n_blocks, c.total = total, c.n_ctas = n_ctas;
+      c.start = at, c.end = at + tk.n_blocks, c.base = base_blocks, c.more = more, c.n_ctas = n_ctas;
       c.tok = tok, c.n_tok = ntok, c.head = head0, c.n_heads = nheads, c.pad = 0;
       P.cuts[blockIdx.x] = c;
     }
@@ -283,7 +303,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) 
           raw[wd][0] = v.x, raw[wd][1] = v.y, raw[wd][2] = v.z, raw[wd][3] = v.w;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 f = P.dtype == SB_DTYPE_BF16 ? unpack_bf2(raw[wd][i]) : unpack_half2(raw[wd][i]);
+            const float2 f = unpack2<T>(raw[wd][i]);
             big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
             sum[wd / WPG] += f.x + f.y;
           }
@@ -298,7 +318,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) 
           float f[8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 v = P.dtype == SB_DTYPE_BF16 ? unpack_bf2(raw[wd][i]) : unpack_half2(raw[wd][i]);
+            const float2 v = unpack2<T>(raw[wd][i]);
             f[2 * i] = v.x * norm, f[2 * i + 1] = v.y * norm;
           }
           // codes 1, 3, 5, 7 of a word enter the products 16 times as large
@@ -323,58 +343,92 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) 
     }
 
     // ---- loads: this warp's keys of block i into stage s
-    const char *kbase = reinterpret_cast<const char *>(A.cache.data) +
-                        (int64_t)g * A.cache.stride_head * (GROUP == 0 ? 2 : 1);
-    const int64_t v_off = A.cache.stride_kv * (GROUP == 0 ? 2 : 1);
-    const char *sbase = reinterpret_cast<const char *>(A.cache.scales) + (int64_t)g * A.cache.scale_head * 2;
-    const bool whole_pages = bs % WK == 0;  // a warp's keys then lie in one page
-    auto page_of = [&](int i) -> int {
-      return i < i1 ? find_block(A.batch, b, (block_key(tk, i, KB) + warp * WK) / bs, A.cache.n_blocks) : -1;
+    constexpr int kElem = GROUP == 0 ? 2 : 1;
+    constexpr int kChunks = R::kRow / 16;    // 16-byte pieces of a row
+    constexpr int kRowsAt = 32 / kChunks;    // rows of one instruction
+    constexpr uint32_t kAll = WK == 32 ? 0xffffffffu : (1u << (WK & 31)) - 1;
+    const int64_t row_bytes = A.cache.stride_pos * kElem, v_off = A.cache.stride_kv * kElem;
+    // this lane's piece of a stage's first rows: source and destination
+    const char *kbase = reinterpret_cast<const char *>(A.cache.data) + (int64_t)g * A.cache.stride_head * kElem +
+                        (lane / kChunks) * row_bytes + (lane % kChunks) * 16;
+    const char *sbase = reinterpret_cast<const char *>(A.cache.scales) + 2 * ((int64_t)g * A.cache.scale_head);
+    const char *table = reinterpret_cast<const char *>(A.batch.block_tables) +
+                        (int64_t)b * A.batch.table_stride * (wide_table ? 8 : 4);
+    auto piece_at = [&](int rr) {  // of row rr, this lane's column
+      // rows: 16-byte pieces exchanged by the row's low bits, so that eight rows of one column
+      // (ldmatrix) lie in different banks
+      const int c = lane % kChunks;
+      return rr * R::kPitch + (GROUP == 0 ? ((c ^ (rr & 7)) << 4) : (c << 4));
     };
-    int next_page = whole_pages ? page_of(i0) : -1;
+    const bool whole_pages = P.page_shift >= 0 ? (1 << P.page_shift) >= WK : bs % WK == 0;  // a warp's keys in one page
+    auto page_of = [&](int key) -> int {
+      const int lb = P.page_shift >= 0 ? key >> P.page_shift : key / bs;
+      if (lb >= A.batch.max_blocks) return -1;
+      const int64_t e = wide_table ? reinterpret_cast<const int64_t *>(table)[lb] : reinterpret_cast<const int32_t *>(table)[lb];
+      return (uint64_t)e < (uint64_t)A.cache.n_blocks ? (int)e : -1;
+    };
+    auto in_page = [&](int key) -> int { return P.page_shift >= 0 ? key & ((1 << P.page_shift) - 1) : key % bs; };
+    int next_page = whole_pages ? page_of(block_key(tk, i0, KB) + warp * WK) : -1;
     auto issue = [&](int i, int s) {
       if (i < i1) {
         const int key0 = block_key(tk, i, KB) + warp * WK;
         const uint32_t dst = ring + s * R::kStage;
-        bool in = lane < WK && in_span(tk.span, key0 + lane);
-        int64_t row = 0, srow = 0;  // bytes, of the lane's key (or of key0 where pages are whole)
+        uint32_t bits = kAll;
         if (whole_pages) {
           const int page = next_page;
-          next_page = page_of(i + 1);  // its latency passes behind this block's work
-          in = in && page >= 0;
-          const int64_t off = key0 % bs;
-          const int64_t pg = max(page, 0);
-          row = pg * A.cache.stride_block + off * A.cache.stride_pos;
-          srow = pg * A.cache.scale_block + off * A.cache.scale_pos;
-        } else if (in) {
-          in = key_row(A, b, key0 + lane, row, srow);
-        }
-        const uint32_t bits = __ballot_sync(0xffffffffu, in);
-        if (lane == 0) seen_bits[warp * 8 + s] = bits;
-        constexpr int kChunks = R::kRow / 16;  // 16-byte pieces of a row
-        const int c = lane % kChunks;
-        constexpr int kRowsAt = 32 / kChunks;  // rows of one instruction
+          // the next page's number is on its way behind this block's work
+          if (i + 1 < i1) next_page = page_of(block_key(tk, i + 1, KB) + warp * WK);
+          const int off = in_page(key0);
+          if (!(page >= 0 && key0 + WK <= tk.span.end && (key0 >= tk.span.first || key0 + WK <= tk.span.sink_end)))
+            bits = __ballot_sync(0xffffffffu, lane < WK && page >= 0 && in_span(tk.span, key0 + lane));
+          const char *src = kbase + (int64_t)max(page, 0) * (A.cache.stride_block * kElem) + off * row_bytes;
+          if (bits == kAll) {
 #pragma unroll
-        for (int it = 0; it < WK / kRowsAt; ++it) {
-          const int rr = it * kRowsAt + lane / kChunks;
-          int64_t off;
-          if (whole_pages) off = row + rr * A.cache.stride_pos;
-          else off = __shfl_sync(0xffffffffu, row, rr);
-          const char *src = kbase + off * (GROUP == 0 ? 2 : 1) + c * 16;
-          const bool take = (bits >> rr) & 1;
-          // rows: 16-byte pieces exchanged by the row's low bits, so that eight rows of one column
-          // (ldmatrix) lie in different banks
-          const uint32_t to = dst + rr * R::kPitch + (GROUP == 0 ? ((c ^ (rr & 7)) << 4) : (c << 4));
-          cp_async16(to, take ? src : kbase, take);
-          cp_async16(to + R::kTile, take ? src + v_off : kbase, take);
+            for (int it = 0; it < WK / kRowsAt; ++it) {
+              const uint32_t to = dst + piece_at(it * kRowsAt + lane / kChunks);
+              cp_async16(to, src);
+              cp_async16(to + R::kTile, src + v_off);
+              src += kRowsAt * row_bytes;
+            }
+          } else {
+#pragma unroll
+            for (int it = 0; it < WK / kRowsAt; ++it) {
+              const int rr = it * kRowsAt + lane / kChunks;
+              const uint32_t to = dst + piece_at(rr);
+              const bool take = (bits >> rr) & 1;
+              cp_async16_or_zero(to, take ? src : kbase, take);
+              cp_async16_or_zero(to + R::kTile, take ? src + v_off : kbase, take);
+              src += kRowsAt * row_bytes;
+            }
+          }
+          if constexpr (GROUP != 0) {
+            const bool in = (bits >> lane) & 1;
+            const char *from = sbase + 2 * ((int64_t)max(page, 0) * A.cache.scale_block + (off + lane) * A.cache.scale_pos);
+            const uint32_t to = dst + WK * R::kPitch + lane * R::kScale;
+            cp_async_small<R::kScale>(to, in ? from : sbase, in);
+            cp_async_small<R::kScale>(to + R::kTile, in ? from + A.cache.scale_kv * 2 : sbase, in);
+          }
+        } else {
+          int64_t row = 0, srow = 0;  // of the lane's key
+          const bool in = lane < WK && in_span(tk.span, key0 + lane) && key_row(A, b, key0 + lane, row, srow);
+          bits = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+          for (int it = 0; it < WK / kRowsAt; ++it) {
+            const int rr = it * kRowsAt + lane / kChunks;
+            const char *src = kbase - (lane / kChunks) * row_bytes + __shfl_sync(0xffffffffu, row, rr) * kElem;
+            const uint32_t to = dst + piece_at(rr);
+            const bool take = (bits >> rr) & 1;
+            cp_async16_or_zero(to, take ? src : kbase, take);
+            cp_async16_or_zero(to + R::kTile, take ? src + v_off : kbase, take);
+          }
+          if constexpr (GROUP != 0) {
+            const char *from = sbase + 2 * srow;
+            const uint32_t to = dst + WK * R::kPitch + lane * R::kScale;
+            cp_async_small<R::kScale>(to, in ? from : sbase, in);
+            cp_async_small<R::kScale>(to + R::kTile, in ? from + A.cache.scale_kv * 2 : sbase, in);
+          }
         }
-        if constexpr (GROUP != 0) {
-          const int64_t off = whole_pages ? srow + lane * A.cache.scale_pos : srow;
-          const char *src = sbase + off * 2;
-          const uint32_t to = dst + WK * R::kPitch + lane * R::kScale;
-          cp_async_small<R::kScale>(to, in ? src : sbase, in);
-          cp_async_small<R::kScale>(to + R::kTile, in ? src + A.cache.scale_kv * 2 : sbase, in);
-        }
+        if (lane == 0) seen_bits[warp * 8 + s] = bits;
       }
       cp_commit();
     };
@@ -411,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) 
       const uint32_t kt = ring + stage * R::kStage, vt = kt + R::kTile;
       const uint8_t *kp = ring_ptr + stage * R::kStage, *vp = kp + R::kTile;
       const int last = key0 + WK - 1;
-      const bool all_seen = bits == (WK == 32 ? 0xffffffffu : (1u << (WK & 31)) - 1) && last <= tk.pmin &&
+      const bool all_seen = bits == kAll && last <= tk.pmin &&
                             (key0 > tk.pmax - A.window || last < A.sinks);
       // ---- S^T: [SUB][NT] tiles of 16 keys x 8 rows
       float sc[SUB][NT][4];
@@ -561,7 +615,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) 
           // times the value it stands for (the zero takes the rest back): far below a bf16 result's
           // rounding, but above an fp16 one's, for which what was dropped enters as a second product.
           uint32_t pb[NT][NG][2], pl[NT][NG][2];
-          const bool fine = P.dtype == SB_DTYPE_F16;
+          constexpr bool fine = std::is_same<T, __half>::value;
 #pragma unroll
           for (int gq = 0; gq < NG; ++gq) {
             const float2 s0 = unpack_half2(*reinterpret_cast<const uint32_t *>(vp + WK * R::kPitch + (16 * j + r) * R::kScale + 4 * gq));
@@ -732,7 +786,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeParams P) 
         if (lane == 0) part[kRows * D + row] = m, part[kRows * D + kRows + row] = l;
       }
     }
-    cur += i1 - i0;
+    cur += P.whole ? 1 : i1 - i0;
     __syncthreads();  // the join buffer becomes the ring again
   }
 }
@@ -746,10 +800,9 @@ __global__ void __launch_bounds__(256) join_kernel(const DecodeParams P, int row
   const int k = blockIdx.x;
   const CutUnit c = P.cuts[k];
   if (k == 0 || k >= c.n_ctas) return;
-  const int64_t mine = cut_at(c.total, c.n_ctas, k), before = cut_at(c.total, c.n_ctas, k - 1);
+  const int64_t mine = cut_at(c.base, c.more, k), before = cut_at(c.base, c.more, k - 1);
   if (mine == c.start || before > c.start) return;
-  int last = k;
-  while (last + 1 < c.n_ctas && cut_at(c.total, c.n_ctas, last + 1) < c.end) ++last;
+  const int last = cta_of(c.base, c.more, c.end - 1);
   const int lane = threadIdx.x % 32;
   const int64_t slot = (int64_t)rows * (D + 2);
   const float *first = P.partials + ((int64_t)(k - 1) * 2 + (before != c.start)) * slot;
@@ -779,17 +832,17 @@ __global__ void __launch_bounds__(256) join_kernel(const DecodeParams P, int row
   }
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-  return n > 0 ? n : 148;
-}
-
 // Rows of a tile: eight where a request's rows fit them, else sixteen.
 int tile_rows(const AttendParams &P) {
   const int64_t per_request = ((int64_t)P.batch.n_tokens + P.batch.batch - 1) / P.batch.batch;
   return P.G * per_request <= 8 ? 8 : 16;
+}
+
+// Tiles of a call, at most, over its KV heads.
+int64_t max_tiles(const DecodeParams &P) {
+  const sb_paged_batch &b = P.a.batch;
+  const int64_t tiles = std::min<int64_t>(b.n_tokens, b.n_tokens / P.tokens_per_tile + b.batch);
+  return tiles * P.head_tiles * P.a.cache.n_heads;
 }
 
 int max_grid(const AttendParams &P, int resident) {
@@ -798,21 +851,18 @@ int max_grid(const AttendParams &P, int resident) {
   const int64_t blocks = ((int64_t)P.batch.max_blocks * P.cache.block_size + 63) / 64 + 1;
   return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)resident * sm_count(), tiles * blocks));
 }
-constexpr int kMaxResident = 4;
-
 template <typename T, int D, int GROUP, int NT>
 int run(const DecodeParams &P, cudaStream_t st) {
   auto kernel = decode_kernel<T, D, GROUP, NT>;
   constexpr int kSmem = smem_bytes<D, GROUP, NT>();
   static_assert(kSmem <= 227 * 1024, "shared memory");
   if (ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), kSmem) != SB_OK) return SB_ERR_CUDA;
-  constexpr int kResident = std::min(kMaxResident, (227 * 1024) / (kSmem + 1024));
-  const int grid = max_grid(P.a, kResident);
+  const int grid = P.whole ? (int)std::min<int64_t>(max_tiles(P), 1 << 20) : max_grid(P.a, resident<D, GROUP, NT>());
   const int slot = prof_before(st);
   kernel<<<grid, kThreads, kSmem, st>>>(P);
   prof_after(slot, st);
   int s = launch_status();
-  if (s != SB_OK || grid == 1) return s;
+  if (s != SB_OK || grid == 1 || P.whole) return s;
   join_kernel<D><<<grid, 256, 0, st>>>(P, 8 * NT);
   return launch_status();
 }
@@ -820,6 +870,11 @@ int run(const DecodeParams &P, cudaStream_t st) {
 template <typename T, int D, int GROUP>
 int by_rows(const DecodeParams &P, int rows, cudaStream_t st) {
   return rows == 8 ? run<T, D, GROUP, 1>(P, st) : run<T, D, GROUP, 2>(P, st);
+}
+
+template <int D, int GROUP>
+int by_type(const DecodeParams &P, int rows, cudaStream_t st) {
+  return P.dtype == SB_DTYPE_BF16 ? by_rows<__nv_bfloat16, D, GROUP>(P, rows, st) : by_rows<__half, D, GROUP>(P, rows, st);
 }
 
 }  // namespace
@@ -849,6 +904,13 @@ int launch_decode(const AttendParams &A, int dtype, void *workspace, cudaStream_
   P.heads_per_tile = std::min(A.G, rows);
   P.tokens_per_tile = rows / P.heads_per_tile;
   P.head_tiles = (A.G + P.heads_per_tile - 1) / P.heads_per_tile;
+  P.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (A.cache.block_size == 1 << i) P.page_shift = i;
+  // Short contexts are not worth a second launch: up to 16 blocks of 64 keys a tile are left whole.
+  const int64_t held = (int64_t)A.batch.max_blocks * A.cache.block_size;
+  const int64_t seen = P.tokens_per_tile == 1 && A.window < 0x7fffffff ? std::min(held, (int64_t)A.window + A.sinks) : held;
+  P.whole = seen <= kWholeKeys;
   // a launch takes at most kMaxRequests requests; later ones of the stream reuse the workspace
   for (int b = 0; b < A.batch.batch; b += kMaxRequests) {
     P.a = A;
@@ -859,15 +921,10 @@ int launch_decode(const AttendParams &A, int dtype, void *workspace, cudaStream_
     int s;
     const int D = A.cache.head_dim;
     switch (A.cache.group) {
-      case 0:
-        if (dtype == SB_DTYPE_BF16)
-          s = D == 128 ? by_rows<__nv_bfloat16, 128, 0>(P, rows, st) : by_rows<__nv_bfloat16, 64, 0>(P, rows, st);
-        else
-          s = D == 128 ? by_rows<__half, 128, 0>(P, rows, st) : by_rows<__half, 64, 0>(P, rows, st);
-        break;
-      case 32: s = D == 128 ? by_rows<__half, 128, 32>(P, rows, st) : by_rows<__half, 64, 32>(P, rows, st); break;
-      case 64: s = D == 128 ? by_rows<__half, 128, 64>(P, rows, st) : by_rows<__half, 64, 64>(P, rows, st); break;
-      default: s = by_rows<__half, 128, 128>(P, rows, st);
+      case 0: s = D == 128 ? by_type<128, 0>(P, rows, st) : by_type<64, 0>(P, rows, st); break;
+      case 32: s = D == 128 ? by_type<128, 32>(P, rows, st) : by_type<64, 32>(P, rows, st); break;
+      case 64: s = D == 128 ? by_type<128, 64>(P, rows, st) : by_type<64, 64>(P, rows, st); break;
+      default: s = by_type<128, 128>(P, rows, st);
     }
     if (s != SB_OK) return s;
   }

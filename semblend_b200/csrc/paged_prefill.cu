@@ -843,12 +843,6 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandPara
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-  return n > 0 ? n : 148;
-}
 
 // Expanded rows: keys of a request, bytes of one KV head (K and V), and how many heads go at a time: what
 // 1 GiB holds, at least one.

@@ -47,9 +47,12 @@ def _need(t, name: str, device: torch.device | None = None) -> None:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
+_HERE = nullcontext()
+
+
 def _on(device: torch.device):
     """The device's context, entered only where it is not the current one."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _inv_freq64(rope_base: float, head_dim: int, device: torch.device) -> torch.Tensor:
@@ -83,27 +86,24 @@ class PagedBatch:
         dev = block_tables.device
         _need(cu_seqlens, "cu_seqlens", dev)
         _need(positions, "positions", dev)
-        if block_tables.ndim != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
-            raise ValueError(f"block_tables must be [B, max_blocks] with contiguous rows, got {tuple(block_tables.shape)}")
+        if block_tables.ndim != 2:
+            raise ValueError(f"block_tables must be [B, max_blocks], got {tuple(block_tables.shape)}")
+        batch, max_blocks = block_tables.shape
+        row, step = block_tables.stride()
+        if batch <= 1:
+            row = max_blocks
+        if (max_blocks > 1 and step != 1) or row < max_blocks:
+            raise ValueError("the rows of block_tables must be contiguous and must not overlap")
         if cu_seqlens.dtype != torch.int32:
             raise TypeError(f"cu_seqlens must be int32, got {cu_seqlens.dtype}")
-        if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] != block_tables.shape[0] + 1 or not cu_seqlens.is_contiguous():
-            raise ValueError(f"cu_seqlens must be a contiguous [{block_tables.shape[0] + 1}] tensor, got {tuple(cu_seqlens.shape)}")
+        if cu_seqlens.shape != (batch + 1,) or not cu_seqlens.is_contiguous():
+            raise ValueError(f"cu_seqlens must be a contiguous [{batch + 1}] tensor, got {tuple(cu_seqlens.shape)}")
         if positions.ndim != 1 or not positions.is_contiguous():
             raise ValueError(f"positions must be a contiguous 1-D tensor, got {tuple(positions.shape)}")
         self.block_tables, self.cu_seqlens, self.positions, self.device = block_tables, cu_seqlens, positions, dev
-        c = _lib.SbPagedBatch()
-        c.block_tables = block_tables.data_ptr()
-        c.cu_seqlens = cu_seqlens.data_ptr()
-        c.positions = positions.data_ptr()
-        c.batch, c.max_blocks = block_tables.shape
-        c.table_stride = block_tables.stride(0) if c.batch > 1 else c.max_blocks
-        if c.table_stride < c.max_blocks:
-            raise ValueError("the rows of block_tables overlap")
-        c.n_tokens = positions.shape[0]
-        c.table_dtype = _lib.index_code(block_tables.dtype)
-        c.pos_dtype = _lib.index_code(positions.dtype)
-        self._c = c
+        self._c = _lib.SbPagedBatch(block_tables.data_ptr(), cu_seqlens.data_ptr(), positions.data_ptr(), row, batch,
+                                    positions.shape[0], max_blocks, _lib.index_code(block_tables.dtype),
+                                    _lib.index_code(positions.dtype), 0)
 
     @property
     def n_tokens(self) -> int:
@@ -141,12 +141,8 @@ class Int4KVCache:
             )
         if codes.stride(4) != 1 or scales.stride(5) != 1 or (scales.shape[4] > 1 and scales.stride(4) != 2):
             raise ValueError("the rows of codes and scales must be contiguous")
-        c = _lib.SbPagedCache()
-        c.data, c.scales = codes.data_ptr(), scales.data_ptr()
-        c.stride_block, c.stride_kv, c.stride_head, c.stride_pos = _axis_strides(codes, layout)
-        c.scale_block, c.scale_kv, c.scale_head, c.scale_pos = _axis_strides(scales, layout)
-        c.n_blocks, c.block_size, c.n_heads, c.head_dim, c.group = nb, bs, nh, self.head_dim, self.group
-        self._c = c
+        self._c = _lib.SbPagedCache(codes.data_ptr(), scales.data_ptr(), *_axis_strides(codes, layout),
+                                    *_axis_strides(scales, layout), nb, bs, nh, self.head_dim, self.group, 0)
 
     @classmethod
     def allocate(cls, num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int, *, group: int = 64,
@@ -172,7 +168,9 @@ class Int4KVCache:
 def _axis_strides(t: torch.Tensor, layout: str) -> tuple[int, int, int, int]:
     """(block, kv, head, position) strides; a dimension of one element may carry any, so it gets 0."""
     shape, stride = t.shape, t.stride()
-    return tuple(0 if shape[a] == 1 else stride[a] for a in _rows._AXES[layout][:4])
+    b, k, h, p, _ = _rows._AXES[layout]
+    return (0 if shape[b] == 1 else stride[b], stride[k], 0 if shape[h] == 1 else stride[h],
+            0 if shape[p] == 1 else stride[p])
 
 
 def _cache(kv_cache, batch: PagedBatch, layout: str) -> _lib.SbPagedCache:
@@ -187,33 +185,28 @@ def _cache(kv_cache, batch: PagedBatch, layout: str) -> _lib.SbPagedCache:
     nb, nh, bs, hd = _rows.paged_geometry(kv_cache.shape, layout)
     if hd > 1 and kv_cache.stride(4) != 1:
         raise ValueError("the rows of kv_cache must be contiguous")
-    c = _lib.SbPagedCache()
-    c.data, c.scales, c.group = kv_cache.data_ptr(), None, 0
-    c.stride_block, c.stride_kv, c.stride_head, c.stride_pos = _axis_strides(kv_cache, layout)
-    c.n_blocks, c.block_size, c.n_heads, c.head_dim = nb, bs, nh, hd
-    c.dtype = _lib.dtype_code(kv_cache.dtype)
-    return c
+    return _lib.SbPagedCache(kv_cache.data_ptr(), None, *_axis_strides(kv_cache, layout), 0, 0, 0, 0, nb, bs, nh, hd, 0,
+                             _lib.dtype_code(kv_cache.dtype))
 
 
 def _token_rows(t: torch.Tensor, name: str, batch: PagedBatch, heads: int | None, head_dim: int,
-                dtype: torch.dtype | None = None) -> _lib.SbTokenRows:
+                dtype: torch.dtype) -> _lib.SbTokenRows:
     """A ``[T, heads, D]`` tensor with contiguous rows."""
     _need(t, name, batch.device)
-    shape = t.shape
-    if len(shape) != 3 or shape[0] != batch._c.n_tokens or shape[2] != head_dim or (heads is not None and shape[1] != heads):
-        raise ValueError(f"{name} must be [{batch._c.n_tokens}, {'heads' if heads is None else heads}, {head_dim}], "
-                         f"got {tuple(shape)}")
-    if dtype is not None and t.dtype != dtype:
+    n = batch._c.n_tokens
+    if t.ndim != 3 or t.shape != (n, t.shape[1] if heads is None else heads, head_dim):
+        raise ValueError(f"{name} must be [{n}, {'heads' if heads is None else heads}, {head_dim}], got {tuple(t.shape)}")
+    if t.dtype != dtype:
         raise TypeError(f"{name} dtype {t.dtype} differs from {dtype}")
-    st = t.stride()
-    if st[2] != 1 and head_dim > 1:
+    token, head, step = t.stride()
+    if step != 1 and head_dim > 1:
         raise ValueError(f"the rows of {name} must be contiguous")
-    return _lib.SbTokenRows(t.data_ptr(), 0 if shape[0] == 1 else st[0], 0 if shape[1] == 1 else st[1])
+    return _lib.SbTokenRows(t.data_ptr(), 0 if n == 1 else token, 0 if t.shape[1] == 1 else head)
 
 
 def _written(t: torch.Tensor, name: str) -> None:
     """An output whose rows lie on one another has no one answer."""
-    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+    if 0 in t.stride() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
         raise ValueError(f"{name} is expanded: its rows share memory")
 
 
