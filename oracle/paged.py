@@ -55,9 +55,8 @@ def rotate(x: torch.Tensor, positions: torch.Tensor, base: float | None, style: 
 def quantise(x: torch.Tensor, group: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Codes and (step, zero) of rows rounded to fp32, each operation rounded to fp32."""
     g = x.float().unflatten(-1, (-1, group))
-    lo, hi = g.amin(-1), g.amax(-1)
-    zero = lo.clamp(-65504, 65504).half()
-    step = ((hi - lo) / 15).clamp(max=65504).half()
+    lo, hi = g.amin(-1).clamp(-60000, 60000), g.amax(-1).clamp(-60000, 60000)
+    zero, step = lo.half(), ((hi - lo) / 15).half()
     inv = torch.where(step.float() > 0, 1.0 / step.float(), torch.zeros(()))
     codes = ((g - zero.float()[..., None]) * inv[..., None]).round().clamp(0, 15).nan_to_num(0.0)
     return codes.flatten(-2).to(torch.uint8), torch.stack([step, zero], -1)

@@ -18,30 +18,31 @@ namespace sb {
 namespace {
 
 using paged::find_block;
-using paged::find_request;
+using paged::find_request_warp;
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 4;  // tokens of a CTA
+constexpr int kMaxTokens = 8;    // tokens of a CTA
+constexpr int kMaxTokens4 = 16;  // 4-bit: a row is four threads, and a block's share of the work is to fill it
 
 // Where a CTA's tokens go; filled by its first threads.
 struct TokenSlot {
-  int64_t position;
   int64_t offset;  // of the row inside the cache (kv 0, head 0), elements or code bytes; -1: none
   int64_t scale_offset;
   int active;      // 0: padding
 };
 
-__device__ __forceinline__ void resolve_token(const sb_paged_cache &C, const sb_paged_batch &B, int t,
+// By a whole warp.
+__device__ __forceinline__ void resolve_token(const sb_paged_cache &C, const sb_paged_batch &B, int page_shift, int t,
                                               TokenSlot &s, unsigned long long *err) {
+  const int64_t p = paged::index_at(B.positions, t, B.pos_dtype);
+  const int b = find_request_warp(B, t);
+  if ((threadIdx.x & 31) != 0) return;
   s.offset = -1;
   s.scale_offset = 0;
-  s.active = 0;
-  const int b = find_request(B, t);
+  s.active = b >= 0;
   if (b < 0) return;
-  const int64_t p = paged::index_at(B.positions, t, B.pos_dtype);
-  s.active = 1;
-  s.position = p;
-  const int64_t lb = p < 0 ? -1 : p / C.block_size;
+  int64_t lb = -1;
+  if (p >= 0) lb = page_shift >= 0 ? p >> page_shift : p / C.block_size;
   const int phys = find_block(B, b, lb, C.n_blocks);
   if (phys < 0) {
     if (err) atomicAdd(err, 1ull);
@@ -52,6 +53,13 @@ __device__ __forceinline__ void resolve_token(const sb_paged_cache &C, const sb_
   s.scale_offset = phys * C.scale_block + in_block * C.scale_pos;
 }
 
+// Rows and tokens that a block of `slots` row slots takes at a time: all rows of a token, and as many tokens
+// as then fit; or, with more rows than slots, equal parts of them.
+struct RowPlan {
+  int rows, tokens;
+  unsigned by_rows;  // reciprocal(rows)
+};
+
 struct AppendParams {
   sb_paged_cache cache;
   sb_paged_batch batch;
@@ -61,7 +69,23 @@ struct AppendParams {
   int n_q_heads;
   int rows;  // rows per token: K heads, V heads, query heads
   int tokens_per_cta;
+  int page_shift, group_shift;  // block_size (-1: none) and group as powers of two
+  unsigned by_rows, by_lanes;  // divisors of thread numbers: reciprocal()
+  RowPlan plan;                // 4-bit caches
 };
+
+// x / d of a thread number x < 256 as x * reciprocal(d) >> 16: exact, since x / 65536 is less than the 1 / d a
+// remainder leaves (d <= 256; a larger d gives 0 either way).
+unsigned reciprocal(int d) { return d > 256 ? 0u : 65536u / (unsigned)d + 1u; }
+RowPlan row_plan(int slots, int all) {
+  const int parts = (all + slots - 1) / slots;
+  RowPlan p;
+  p.rows = (all + parts - 1) / parts;
+  p.tokens = slots / p.rows;
+  p.by_rows = reciprocal(p.rows);
+  return p;
+}
+__device__ __forceinline__ int thread_div(int x, unsigned r) { return (int)((unsigned)x * r >> 16); }
 
 // cos and sin of p * f to fp32: the turn is reduced to [-1/2, 1/2] in 64 bits
 // (positions reach millions of radians, where an fp32 angle has lost its
@@ -75,95 +99,140 @@ __device__ __forceinline__ float2 turn(int64_t p, double f) {
   return cs;
 }
 
-template <typename T, int VEC, bool ROTATE, bool NEOX>
-__device__ __forceinline__ void move_row(const T *src, T *dst, int lane, int half, const float2 *cs) {
-  // two vectors of the row: its RoPE pairs lie across them (neox) or inside each (interleaved)
-  const int d0 = (VEC == 1 && !NEOX) ? 2 * lane : lane * VEC;
-  const int d1 = (VEC == 1 && !NEOX) ? 2 * lane + 1 : half + lane * VEC;
-  Vec<T, VEC> a, b;
-  load_vec(a, src + d0);
-  load_vec(b, src + d1);
-  if (ROTATE) {
-    if (NEOX || VEC == 1) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float2 w = cs[lane * VEC + i];
-        const float x = Elem<T>::to_f32(a.e[i]), y = Elem<T>::to_f32(b.e[i]);
-        a.e[i] = Elem<T>::from_f32(x * w.x - y * w.y);
-        b.e[i] = Elem<T>::from_f32(y * w.x + x * w.y);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i + 1 < VEC; i += 2) {
-        const float2 w = cs[(d0 + i) / 2], u = cs[(d1 + i) / 2];
-        const float x = Elem<T>::to_f32(a.e[i]), y = Elem<T>::to_f32(a.e[i + 1]);
-        const float p = Elem<T>::to_f32(b.e[i]), q = Elem<T>::to_f32(b.e[i + 1]);
-        a.e[i] = Elem<T>::from_f32(x * w.x - y * w.y);
-        a.e[i + 1] = Elem<T>::from_f32(y * w.x + x * w.y);
-        b.e[i] = Elem<T>::from_f32(p * u.x - q * u.y);
-        b.e[i + 1] = Elem<T>::from_f32(q * u.x + p * u.y);
-      }
-    }
+// A thread's place in the line of a CTA's rows (token by token), moved on by
+// whole steps without a division.
+struct RowCursor {
+  int token, row;
+  __device__ __forceinline__ RowCursor(int first, int rows, unsigned by_rows)
+      : token(thread_div(first, by_rows)), row(first - thread_div(first, by_rows) * rows) {}
+  __device__ __forceinline__ void advance(int step, int rows) {
+    row += step;
+    while (row >= rows) row -= rows, ++token;
   }
-  store_vec(dst + d0, a);
-  store_vec(dst + d1, b);
-}
+};
 
 template <typename T, int VEC, bool NEOX>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams P) {
+__global__ void __launch_bounds__(kThreads, 8) append_kernel(const AppendParams P) {
   __shared__ TokenSlot slot[kMaxTokens];
   __shared__ float2 cs[kMaxTokens][256];  // head_dim <= 512
   const int D = P.cache.head_dim, half = D / 2, H = P.cache.n_heads;
   const int t0 = blockIdx.x * P.tokens_per_cta;
   const int n = min(P.tokens_per_cta, P.batch.n_tokens - t0);
-  if (threadIdx.x < n) resolve_token(P.cache, P.batch, t0 + threadIdx.x, slot[threadIdx.x], P.err);
+  const int lanes = half / VEC;  // threads a row
+  const int mine = thread_div(threadIdx.x, P.by_lanes), lane = threadIdx.x - mine * lanes;
+  const int step = kThreads / lanes;
+  RowCursor at(mine, P.rows, P.by_rows);
+  const bool idle = mine >= step;  // lanes does not divide the block: the last threads have no row
+  // two vectors of the row: its RoPE pairs lie across them (neox) or inside each (interleaved)
+  const int d0 = (VEC == 1 && !NEOX) ? 2 * lane : lane * VEC;
+  const int d1 = (VEC == 1 && !NEOX) ? 2 * lane + 1 : half + lane * VEC;
+  Vec<T, VEC> a, b;
+  auto load = [&] {
+    const int kv = at.row >= H, q = at.row >= 2 * H;
+    const int h = at.row - (kv + q) * H;
+    const T *from = reinterpret_cast<const T *>(q ? P.query.data : kv ? P.value.data : P.key.data) +
+                    (t0 + at.token) * (q ? P.query.stride_token : kv ? P.value.stride_token : P.key.stride_token) +
+                    h * (q ? P.query.stride_head : kv ? P.value.stride_head : P.key.stride_head);
+    load_vec(a, from + d0);
+    load_vec(b, from + d1);
+  };
+  if (!idle && at.token < n) load();  // on its way while the tokens' places and angles are found
+  for (int k = threadIdx.x / 32; k < n; k += blockDim.x / 32) resolve_token(P.cache, P.batch, P.page_shift, t0 + k, slot[k], P.err);
   if (P.inv_freq != nullptr)
-    for (int i = threadIdx.x; i < n * half; i += blockDim.x) {
-      const int k = i / half, c = i - k * half;
-      cs[k][c] = turn(paged::index_at(P.batch.positions, t0 + k, P.batch.pos_dtype), P.inv_freq[c]);
+    for (int k = 0, c = threadIdx.x; k < n; c += kThreads) {
+      while (c >= half && k < n) c -= half, ++k;
+      if (k < n) cs[k][c] = turn(paged::index_at(P.batch.positions, t0 + k, P.batch.pos_dtype), P.inv_freq[c]);
     }
   __syncthreads();
-  const int lanes = half / VEC;  // threads a row
-  const int lane = threadIdx.x % lanes, first = threadIdx.x / lanes, step = blockDim.x / lanes;
-  if (first >= step) return;  // lanes does not divide the block: the last threads have no row
-  for (int r = first; r < n * P.rows; r += step) {
-    const int k = r / P.rows, row = r - k * P.rows;
-    const TokenSlot &s = slot[k];
-    if (!s.active) continue;
-    const int64_t t = t0 + k;
-    if (row < 2 * H) {
-      if (s.offset < 0) continue;
-      const int kv = row >= H, h = row - kv * H;
-      const sb_token_rows &src = kv ? P.value : P.key;
-      const T *from = reinterpret_cast<const T *>(src.data) + t * src.stride_token + h * src.stride_head;
-      T *to = reinterpret_cast<T *>(P.cache.data) + s.offset + kv * P.cache.stride_kv + h * P.cache.stride_head;
-      if (kv || P.inv_freq == nullptr) move_row<T, VEC, false, NEOX>(from, to, lane, half, cs[k]);
-      else move_row<T, VEC, true, NEOX>(from, to, lane, half, cs[k]);
-    } else {
-      const int h = row - 2 * H;
-      const T *from = reinterpret_cast<const T *>(P.query.data) + t * P.query.stride_token + h * P.query.stride_head;
-      T *to = reinterpret_cast<T *>(P.query_out.data) + t * P.query_out.stride_token + h * P.query_out.stride_head;
-      if (P.inv_freq == nullptr) move_row<T, VEC, false, NEOX>(from, to, lane, half, cs[k]);
-      else move_row<T, VEC, true, NEOX>(from, to, lane, half, cs[k]);
+  if (idle) return;
+  while (at.token < n) {
+    const TokenSlot &s = slot[at.token];
+    const int kv = at.row >= H, q = at.row >= 2 * H, h = at.row - (kv + q) * H;
+    if (s.active && (q || s.offset >= 0)) {
+      if (P.inv_freq != nullptr && (q || !kv)) {
+        const float2 *w = cs[at.token];
+        if (NEOX || VEC == 1) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float2 u = w[lane * VEC + i];
+            const float x = Elem<T>::to_f32(a.e[i]), y = Elem<T>::to_f32(b.e[i]);
+            a.e[i] = Elem<T>::from_f32(x * u.x - y * u.y);
+            b.e[i] = Elem<T>::from_f32(y * u.x + x * u.y);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i + 1 < VEC; i += 2) {
+            const float2 u = w[(d0 + i) / 2], v = w[(d1 + i) / 2];
+            const float x = Elem<T>::to_f32(a.e[i]), y = Elem<T>::to_f32(a.e[i + 1]);
+            const float z = Elem<T>::to_f32(b.e[i]), r = Elem<T>::to_f32(b.e[i + 1]);
+            a.e[i] = Elem<T>::from_f32(x * u.x - y * u.y);
+            a.e[i + 1] = Elem<T>::from_f32(y * u.x + x * u.y);
+            b.e[i] = Elem<T>::from_f32(z * v.x - r * v.y);
+            b.e[i + 1] = Elem<T>::from_f32(r * v.x + z * v.y);
+          }
+        }
+      }
+      T *to = q ? reinterpret_cast<T *>(P.query_out.data) + (int64_t)(t0 + at.token) * P.query_out.stride_token +
+                      h * P.query_out.stride_head
+                : reinterpret_cast<T *>(P.cache.data) + s.offset + kv * P.cache.stride_kv + h * P.cache.stride_head;
+      store_vec(to + d0, a);
+      store_vec(to + d1, b);
     }
+    at.advance(step, P.rows);
+    if (at.token < n) load();
   }
 }
 
 // ---------------------------------------------------------------------------
 // 4-bit cache
 // ---------------------------------------------------------------------------
-// A row belongs to head_dim / 16 threads; thread j holds elements [8j, 8j + 8)
-// and [D/2 + 8j, D/2 + 8j + 8).  A group is then whole threads of one half, or
+// A row belongs to head_dim / 32 threads; thread j holds elements [16j, 16j + 16)
+// and [D/2 + 16j, D/2 + 16j + 16).  A group is then whole threads of one half, or
 // (group == head_dim) both halves of all of the row's threads.
-__device__ __forceinline__ uint32_t pack_codes(const float (&x)[8], float zero, float inv) {
+constexpr int kPer = 16;
+
+__device__ __forceinline__ uint32_t pack_codes(const float *x, float zero, float inv) {
+  // one rounding each, so that the codes are a function of the fp32 values alone; adding 2^23 rounds to the
+  // nearest integer (ties to even) and leaves it in the lowest bits, and the words' upper bits add up to a
+  // constant (conversions to integer run at an eighth of the rate)
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // one rounding each, so that the codes are a function of the fp32 values alone
-    const float c = rintf(__fmul_rn(__fsub_rn(x[i], zero), inv));
-    w |= (uint32_t)fminf(fmaxf(c, 0.f), 15.f) << (4 * i);
+  for (int i = 7; i >= 0; --i) {
+    const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], zero), inv), 0.f), 15.f);
+    w = w * 16 + __float_as_uint(__fadd_rn(c, 8388608.f));
   }
-  return w;
+  return w - 0x4B000000u * 0x11111111u;
+}
+
+// cos and sin of p * f to about 2^-52: the angle less its nearest multiple of
+// pi / 2 (pi / 2 in two doubles), then the Taylor series up to r^16, whose rest
+// is below 3e-18 for |r| <= pi / 4, and the quadrant's exchange and signs.
+// (sincos() costs several times as much and is exact to the last bit, which
+// the fp32 values made from this do not need.)
+__device__ __forceinline__ double2 turn64(int64_t p, double f) {
+  constexpr double kPiHalf = 1.5707963267948966, kPiHalfRest = 6.123233995736766e-17;
+  const double t = (double)p * f;
+  const double k = rint(t * 0.63661977236758134);
+  const double r = fma(-k, kPiHalfRest, fma(-k, kPiHalf, t));
+  const double x = r * r;
+  double s = fma(x, -1.0 / 1307674368000.0, 1.0 / 6227020800.0);
+  s = fma(x, s, -1.0 / 39916800.0);
+  s = fma(x, s, 1.0 / 362880.0);
+  s = fma(x, s, -1.0 / 5040.0);
+  s = fma(x, s, 1.0 / 120.0);
+  s = fma(x, s, -1.0 / 6.0);
+  s = fma(x * r, s, r);
+  double c = fma(x, 1.0 / 20922789888000.0, -1.0 / 87178291200.0);
+  c = fma(x, c, 1.0 / 479001600.0);
+  c = fma(x, c, -1.0 / 3628800.0);
+  c = fma(x, c, 1.0 / 40320.0);
+  c = fma(x, c, -1.0 / 720.0);
+  c = fma(x, c, 1.0 / 24.0);
+  c = fma(x, c, -0.5);
+  c = fma(x, c, 1.0);
+  const int quadrant = (int)((long long)k & 3);
+  const double u = quadrant & 1 ? s : c, v = quadrant & 1 ? c : s;
+  return make_double2((quadrant + 1) & 2 ? -u : u, quadrant & 2 ? -v : v);
 }
 
 // NaN in, NaN out: a group that holds one reads back as NaN.
@@ -177,12 +246,18 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-__device__ __forceinline__ float saturate_half(float x) { return min_nan(max_nan(x, -65504.f), 65504.f); }
+// Extremes are limited so that every value a group can stand for is finite in fp16.
+__device__ __forceinline__ float saturate(float x) { return min_nan(max_nan(x, -60000.f), 60000.f); }
+
+__device__ __forceinline__ void extend(float (&lo)[2], float (&hi)[2], int k, float x) {
+  lo[k] = min_nan(lo[k], x), hi[k] = max_nan(hi[k], x);
+}
 
 // step and zero of a group from its extremes, and 1 / step (0 for a group of equal values)
 __device__ __forceinline__ __half2 group_scale(float lo, float hi, float &zero, float &inv) {
-  const __half z = __float2half_rn(saturate_half(lo));
-  const __half st = __float2half_rn(min_nan(__fdiv_rn(__fsub_rn(hi, lo), 15.f), 65504.f));
+  lo = saturate(lo), hi = saturate(hi);
+  const __half z = __float2half_rn(lo);
+  const __half st = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
   zero = __half2float(z);
   const float s = __half2float(st);
   inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
@@ -190,11 +265,11 @@ __device__ __forceinline__ __half2 group_scale(float lo, float hi, float &zero, 
 }
 
 template <typename T>
-__device__ __forceinline__ void load8(float (&x)[8], const T *p, bool aligned) {
+__device__ __forceinline__ void load_part(float (&x)[kPer], const T *p, bool aligned) {
   if (aligned) {
     constexpr int kV = 16 / sizeof(T);
 #pragma unroll
-    for (int v = 0; v < 8 / kV; ++v) {
+    for (int v = 0; v < kPer / kV; ++v) {
       Vec<T, kV> a;
       load_vec(a, p + v * kV);
 #pragma unroll
@@ -202,7 +277,7 @@ __device__ __forceinline__ void load8(float (&x)[8], const T *p, bool aligned) {
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = Elem<T>::to_f32(p[i]);
+    for (int i = 0; i < kPer; ++i) x[i] = Elem<T>::to_f32(p[i]);
   }
 }
 
@@ -213,95 +288,106 @@ __device__ __forceinline__ void turn_pair(float &x, float &y, double2 w) {
   y = (float)(b * w.x + a * w.y);
 }
 
-template <typename T, bool NEOX>
+template <typename T, bool NEOX, int D>
 __global__ void __launch_bounds__(kThreads) append4_kernel(const AppendParams P, const bool aligned) {
-  __shared__ TokenSlot slot[kMaxTokens];
-  __shared__ double2 cs[kMaxTokens][64];
-  const int D = P.cache.head_dim, half = D / 2, H = P.cache.n_heads;
+  __shared__ TokenSlot slot[kMaxTokens4];
+  __shared__ double2 cs[kMaxTokens4][64];
+  constexpr int half = D / 2;
+  const int H = P.cache.n_heads;
   const int t0 = blockIdx.x * P.tokens_per_cta;
   const int n = min(P.tokens_per_cta, P.batch.n_tokens - t0);
-  if (threadIdx.x < n) resolve_token(P.cache, P.batch, t0 + threadIdx.x, slot[threadIdx.x], P.err);
+  for (int k = threadIdx.x / 32; k < n; k += blockDim.x / 32) resolve_token(P.cache, P.batch, P.page_shift, t0 + k, slot[k], P.err);
   if (P.inv_freq != nullptr)
-    for (int i = threadIdx.x; i < n * half; i += blockDim.x) {
-      const int k = i / half, c = i - k * half;
-      double2 w;
-      sincos((double)paged::index_at(P.batch.positions, t0 + k, P.batch.pos_dtype) * P.inv_freq[c], &w.y, &w.x);
-      cs[k][c] = w;
+    for (int i = threadIdx.x; i < n * half; i += kThreads) {
+      const int k = i / half, c = i % half;  // half is a power of two
+      cs[k][c] = turn64(paged::index_at(P.batch.positions, t0 + k, P.batch.pos_dtype), P.inv_freq[c]);
     }
   __syncthreads();
-  const int lanes = D / 16;  // 4 or 8 threads a row: whole rows in a warp
-  const int lane = threadIdx.x % lanes, first = threadIdx.x / lanes, step = kThreads / lanes;
+  constexpr int lanes = D / (2 * kPer);  // 2 or 4 threads a row: whole rows in a warp
+  const int lane = threadIdx.x % lanes;
   const int group = P.cache.group;
-  const int total = n * P.rows;
-  // every thread of a warp takes the same number of turns (the shuffles need all of them)
-  for (int r0 = 0; r0 < total; r0 += step) {
-    const int r = r0 + first;
-    const int k = min(r / P.rows, n - 1), row = r - k * P.rows;
-    const TokenSlot &s = slot[k];
-    const bool live = r < total && s.active;
+  const bool one = group == D;  // both halves are one group
+  const int span = one ? lanes : group / kPer;
+  // A thread keeps its row (head and kind) and goes through the tokens; every thread of a warp takes the same
+  // number of turns (the shuffles need all of them).
+  const RowPlan plan = P.plan;
+  const int my_token = thread_div(threadIdx.x / lanes, plan.by_rows), my_row = threadIdx.x / lanes - my_token * plan.rows;
+  for (int row0 = 0; row0 < P.rows; row0 += plan.rows) {
+    const int row = row0 + my_row;
+    const bool row_in = row < P.rows && my_token < plan.tokens;
     const bool is_q = row >= 2 * H;
     const int kv = row >= H, h = is_q ? row - 2 * H : row - kv * H;
-    const bool write = live && (is_q || s.offset >= 0);
-    float a[8], b[8];
-    const sb_token_rows &src = is_q ? P.query : kv ? P.value : P.key;
-    if (write) {
-      const T *from = reinterpret_cast<const T *>(src.data) + (int64_t)(t0 + k) * src.stride_token + h * src.stride_head;
-      load8(a, from + lane * 8, aligned);
-      load8(b, from + half + lane * 8, aligned);
-      if (P.inv_freq != nullptr && (is_q || !kv)) {
-        if (NEOX) {
+    const int64_t from_token = is_q ? P.query.stride_token : kv ? P.value.stride_token : P.key.stride_token;
+    const T *from_row = reinterpret_cast<const T *>(is_q ? P.query.data : kv ? P.value.data : P.key.data) +
+                        h * (is_q ? P.query.stride_head : kv ? P.value.stride_head : P.key.stride_head) + t0 * from_token +
+                        lane * kPer;
+    uint8_t *codes_row = reinterpret_cast<uint8_t *>(P.cache.data) + kv * P.cache.stride_kv + h * P.cache.stride_head +
+                         lane * (kPer / 2);
+    __half *scales_row = reinterpret_cast<__half *>(P.cache.scales) + kv * P.cache.scale_kv + h * P.cache.scale_head;
+    const bool rotate = P.inv_freq != nullptr && (is_q || !kv);
+    for (int k0 = 0; k0 < n; k0 += plan.tokens) {
+      const int k = min(k0 + my_token, n - 1);
+      const TokenSlot &s = slot[k];
+      const bool write = row_in && k0 + my_token < n && s.active && (is_q || s.offset >= 0);
+      float a[kPer], b[kPer];
+      if (write) {
+        const T *from = from_row + k * from_token;
+        load_part(a, from, aligned);
+        load_part(b, from + half, aligned);
+        if (rotate) {
+          const double2 *w = cs[k];
+          if (NEOX) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) turn_pair(a[i], b[i], cs[k][lane * 8 + i]);
-        } else {
+            for (int i = 0; i < kPer; ++i) turn_pair(a[i], b[i], w[lane * kPer + i]);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            turn_pair(a[i], a[i + 1], cs[k][(lane * 8 + i) / 2]);
-            turn_pair(b[i], b[i + 1], cs[k][(half + lane * 8 + i) / 2]);
+            for (int i = 0; i < kPer; i += 2) {
+              turn_pair(a[i], a[i + 1], w[(lane * kPer + i) / 2]);
+              turn_pair(b[i], b[i + 1], w[(half + lane * kPer + i) / 2]);
+            }
           }
         }
-      }
-      if (is_q) {
-        T *to = reinterpret_cast<T *>(P.query_out.data) + (int64_t)(t0 + k) * P.query_out.stride_token +
-                h * P.query_out.stride_head;
+        if (is_q) {
+          T *to = reinterpret_cast<T *>(P.query_out.data) + (t0 + k) * P.query_out.stride_token +
+                  h * P.query_out.stride_head + lane * kPer;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          to[lane * 8 + i] = Elem<T>::from_f32(a[i]);
-          to[half + lane * 8 + i] = Elem<T>::from_f32(b[i]);
+          for (int i = 0; i < kPer; ++i) {
+            to[i] = Elem<T>::from_f32(a[i]);
+            to[half + i] = Elem<T>::from_f32(b[i]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) a[i] = b[i] = 0.f;
+      }
+      float lo[2] = {a[0], b[0]}, hi[2] = {a[0], b[0]};
+#pragma unroll
+      for (int i = 1; i < kPer; ++i) extend(lo, hi, 0, a[i]), extend(lo, hi, 1, b[i]);
+      if (one) extend(lo, hi, 0, lo[1]), extend(lo, hi, 0, hi[1]);
+      for (int o = 1; o < span; o <<= 1) {
+        lo[0] = min_nan(lo[0], __shfl_xor_sync(0xffffffffu, lo[0], o));
+        hi[0] = max_nan(hi[0], __shfl_xor_sync(0xffffffffu, hi[0], o));
+        if (!one) {
+          lo[1] = min_nan(lo[1], __shfl_xor_sync(0xffffffffu, lo[1], o));
+          hi[1] = max_nan(hi[1], __shfl_xor_sync(0xffffffffu, hi[1], o));
         }
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
-    }
-    float lo0 = a[0], hi0 = a[0], lo1 = b[0], hi1 = b[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) {
-      lo0 = min_nan(lo0, a[i]), hi0 = max_nan(hi0, a[i]);
-      lo1 = min_nan(lo1, b[i]), hi1 = max_nan(hi1, b[i]);
-    }
-    if (group == D) {
-      lo0 = lo1 = min_nan(lo0, lo1);
-      hi0 = hi1 = max_nan(hi0, hi1);
-    }
-    const int span = group == D ? lanes : group / 8;
-    for (int o = 1; o < span; o <<= 1) {
-      lo0 = min_nan(lo0, __shfl_xor_sync(0xffffffffu, lo0, o)), hi0 = max_nan(hi0, __shfl_xor_sync(0xffffffffu, hi0, o));
-      lo1 = min_nan(lo1, __shfl_xor_sync(0xffffffffu, lo1, o)), hi1 = max_nan(hi1, __shfl_xor_sync(0xffffffffu, hi1, o));
-    }
-    if (!write || is_q) continue;
-    float zero0, inv0, zero1, inv1;
-    const __half2 s0 = group_scale(lo0, hi0, zero0, inv0), s1 = group_scale(lo1, hi1, zero1, inv1);
-    uint8_t *codes = reinterpret_cast<uint8_t *>(P.cache.data) + s.offset + kv * P.cache.stride_kv +
-                     h * P.cache.stride_head;
-    *reinterpret_cast<uint32_t *>(codes + lane * 4) = pack_codes(a, zero0, inv0);
-    *reinterpret_cast<uint32_t *>(codes + half / 2 + lane * 4) = pack_codes(b, zero1, inv1);
-    __half2 *scales = reinterpret_cast<__half2 *>(reinterpret_cast<__half *>(P.cache.scales) + s.scale_offset +
-                                                  kv * P.cache.scale_kv + h * P.cache.scale_head);
-    if (group == D) {
-      if (lane == 0) scales[0] = s0;
-    } else if (lane % span == 0) {
-      scales[lane * 8 / group] = s0;
-      scales[(half + lane * 8) / group] = s1;
+      if (!write || is_q) continue;
+      float zero0, inv0, zero1, inv1;
+      const __half2 s0 = group_scale(lo[0], hi[0], zero0, inv0);
+      __half2 s1 = s0;
+      zero1 = zero0, inv1 = inv0;
+      if (!one) s1 = group_scale(lo[1], hi[1], zero1, inv1);
+      uint2 *codes = reinterpret_cast<uint2 *>(codes_row + s.offset);
+      codes[0] = make_uint2(pack_codes(a, zero0, inv0), pack_codes(a + 8, zero0, inv0));
+      codes[half / 16] = make_uint2(pack_codes(b, zero1, inv1), pack_codes(b + 8, zero1, inv1));
+      __half2 *scales = reinterpret_cast<__half2 *>(scales_row + s.scale_offset);
+      if (one) {
+        if (lane == 0) scales[0] = s0;
+      } else if ((lane & (span - 1)) == 0) {
+        scales[lane * kPer >> P.group_shift] = s0;
+        scales[(half + lane * kPer) >> P.group_shift] = s1;
+      }
     }
   }
 }
@@ -315,6 +401,9 @@ struct GatherParams {
   sb_token_rows out[2];
   unsigned long long *err;
   int tokens_per_cta;
+  int page_shift, group_shift;
+  unsigned by_rows, by_lanes;
+  RowPlan plan;
 };
 
 template <typename T, int VEC>
@@ -323,12 +412,14 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherParams P) 
   const int H = P.cache.n_heads, rows = 2 * H;
   const int t0 = blockIdx.x * P.tokens_per_cta;
   const int n = min(P.tokens_per_cta, P.batch.n_tokens - t0);
-  if (threadIdx.x < n) resolve_token(P.cache, P.batch, t0 + threadIdx.x, slot[threadIdx.x], P.err);
+  for (int k = threadIdx.x / 32; k < n; k += blockDim.x / 32) resolve_token(P.cache, P.batch, P.page_shift, t0 + k, slot[k], P.err);
   __syncthreads();
   const int lanes = P.cache.head_dim / VEC;
-  for (int i = threadIdx.x; i < n * rows * lanes; i += kThreads) {
-    const int r = i / lanes, lane = i - r * lanes;
-    const int k = r / rows, row = r - k * rows;
+  const int mine = thread_div(threadIdx.x, P.by_lanes), lane = threadIdx.x - mine * lanes;
+  const int step = kThreads / lanes;
+  if (mine >= step) return;
+  for (RowCursor at(mine, rows, P.by_rows); at.token < n; at.advance(step, rows)) {
+    const int k = at.token, row = at.row;
     const TokenSlot &s = slot[k];
     if (s.offset < 0) continue;
     const int kv = row >= H, h = row - kv * H;
@@ -342,47 +433,60 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherParams P) 
 }
 
 // A thread expands 8 codes (4 bytes) of one group to 8 elements.
-template <typename T>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) gather4_kernel(const GatherParams P, const bool aligned) {
-  __shared__ TokenSlot slot[kMaxTokens];
+  __shared__ TokenSlot slot[kMaxTokens4];
   const int H = P.cache.n_heads, rows = 2 * H;
   const int t0 = blockIdx.x * P.tokens_per_cta;
   const int n = min(P.tokens_per_cta, P.batch.n_tokens - t0);
-  if (threadIdx.x < n) resolve_token(P.cache, P.batch, t0 + threadIdx.x, slot[threadIdx.x], P.err);
+  for (int k = threadIdx.x / 32; k < n; k += blockDim.x / 32) resolve_token(P.cache, P.batch, P.page_shift, t0 + k, slot[k], P.err);
   __syncthreads();
-  const int lanes = P.cache.head_dim / 8;
-  for (int i = threadIdx.x; i < n * rows * lanes; i += kThreads) {
-    const int r = i / lanes, lane = i - r * lanes;
-    const int k = r / rows, row = r - k * rows;
-    const TokenSlot &s = slot[k];
-    if (s.offset < 0) continue;
+  constexpr int lanes = D / 8;
+  const int lane = threadIdx.x % lanes;
+  const RowPlan plan = P.plan;
+  const int my_token = thread_div(threadIdx.x / lanes, plan.by_rows), my_row = threadIdx.x / lanes - my_token * plan.rows;
+  if (my_token >= plan.tokens) return;
+  for (int row = my_row; row < rows; row += plan.rows) {
     const int kv = row >= H, h = row - kv * H;
-    const uint8_t *codes = reinterpret_cast<const uint8_t *>(P.cache.data) + s.offset + kv * P.cache.stride_kv +
-                           h * P.cache.stride_head;
-    const __half2 *scales = reinterpret_cast<const __half2 *>(reinterpret_cast<const __half *>(P.cache.scales) +
-                                                              s.scale_offset + kv * P.cache.scale_kv +
-                                                              h * P.cache.scale_head);
-    const uint32_t w = *reinterpret_cast<const uint32_t *>(codes + lane * 4);
-    const float2 sz = __half22float2(scales[lane * 8 / P.cache.group]);
-    T *to = reinterpret_cast<T *>(P.out[kv].data) + (int64_t)(t0 + k) * P.out[kv].stride_token +
-            h * P.out[kv].stride_head + lane * 8;
-    T v[8];
+    const uint8_t *codes = reinterpret_cast<const uint8_t *>(P.cache.data) + kv * P.cache.stride_kv +
+                           h * P.cache.stride_head + lane * 4;
+    const __half *scales = reinterpret_cast<const __half *>(P.cache.scales) + kv * P.cache.scale_kv +
+                           h * P.cache.scale_head + 2 * (lane * 8 >> P.group_shift);
+    const int64_t to_token = kv ? P.out[1].stride_token : P.out[0].stride_token;
+    T *out = reinterpret_cast<T *>(kv ? P.out[1].data : P.out[0].data) +
+             h * (kv ? P.out[1].stride_head : P.out[0].stride_head) + t0 * to_token + lane * 8;
+    for (int k = my_token; k < n; k += plan.tokens) {
+      const TokenSlot &s = slot[k];
+      if (s.offset < 0) continue;
+      const uint32_t w = *reinterpret_cast<const uint32_t *>(codes + s.offset);
+      const float2 sz = __half22float2(*reinterpret_cast<const __half2 *>(scales + s.scale_offset));
+      T *to = out + k * to_token;
+      T v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = Elem<T>::from_f32(fmaf((float)((w >> (4 * j)) & 15u), sz.x, sz.y));
-    if (aligned) {
-      constexpr int kV = 16 / sizeof(T);
+      for (int j = 0; j < 8; ++j) {
+        // 2^23 + code, brought back to the code exactly
+        const float c = __fsub_rn(__uint_as_float(((w >> (4 * j)) & 15u) | 0x4B000000u), 8388608.f);
+        v[j] = Elem<T>::from_f32(fmaf(c, sz.x, sz.y));
+      }
+      if (aligned) {
+        constexpr int kV = 16 / sizeof(T);
 #pragma unroll
-      for (int j = 0; j < 8; j += kV) store_vec(to + j, *reinterpret_cast<const Vec<T, kV> *>(v + j));
-    } else {
+        for (int j = 0; j < 8; j += kV) store_vec(to + j, *reinterpret_cast<const Vec<T, kV> *>(v + j));
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) to[j] = v[j];
+        for (int j = 0; j < 8; ++j) to[j] = v[j];
+      }
     }
   }
 }
 
-// Tokens a CTA takes: one while that leaves SMs without work, else four (the angles of four
-// tokens of head_dim 128 are one per thread).
-int tokens_per_cta(int n_tokens) { return n_tokens >= 4 * kMaxTokens * paged::sm_count() ? kMaxTokens : 1; }
+// Tokens a CTA takes: one while more would leave SMs with a single CTA, up to eight (finding a token's place
+// and angles is then shared by as much of the work as fits the block).
+int tokens_per_cta(int n_tokens, bool codes) {
+  return std::min(codes ? kMaxTokens4 : kMaxTokens, std::max(1, n_tokens / (2 * paged::sm_count())));
+}
+
+using paged::page_shift;
 
 template <typename T, int VEC>
 void launch_append(const AppendParams &P, bool neox, int grid, cudaStream_t st) {
@@ -392,13 +496,14 @@ void launch_append(const AppendParams &P, bool neox, int grid, cudaStream_t st) 
 
 // The widest vector every row of the call can be moved in: 16 bytes, or one element.
 template <typename T>
-int append_rows(const AppendParams &P, bool neox, int grid, cudaStream_t st) {
+int append_rows(AppendParams &P, bool neox, int grid, cudaStream_t st) {
   constexpr int kV = 16 / (int)sizeof(T);
   const int es = (int)sizeof(T);
   const bool wide = (P.cache.head_dim / 2) % kV == 0 && paged::cache_aligned(P.cache, es, 16) &&
                     paged::rows_aligned(P.key, es, 16) && paged::rows_aligned(P.value, es, 16) &&
                     paged::rows_aligned(P.query, es, 16) && paged::rows_aligned(P.query_out, es, 16);
   const int slot = prof_before(st);
+  P.by_lanes = reciprocal(P.cache.head_dim / 2 / (wide ? kV : 1));
   if (wide) launch_append<T, kV>(P, neox, grid, st);
   else launch_append<T, 1>(P, neox, grid, st);
   prof_after(slot, st);
@@ -410,22 +515,33 @@ int append_codes(const AppendParams &P, bool neox, int grid, cudaStream_t st) {
   const bool wide = paged::rows_aligned(P.key, sizeof(T), 16) && paged::rows_aligned(P.value, sizeof(T), 16) &&
                     paged::rows_aligned(P.query, sizeof(T), 16);
   const int slot = prof_before(st);
-  if (neox) append4_kernel<T, true><<<grid, kThreads, 0, st>>>(P, wide);
-  else append4_kernel<T, false><<<grid, kThreads, 0, st>>>(P, wide);
+  if (P.cache.head_dim == 128) {
+    if (neox) append4_kernel<T, true, 128><<<grid, kThreads, 0, st>>>(P, wide);
+    else append4_kernel<T, false, 128><<<grid, kThreads, 0, st>>>(P, wide);
+  } else {
+    if (neox) append4_kernel<T, true, 64><<<grid, kThreads, 0, st>>>(P, wide);
+    else append4_kernel<T, false, 64><<<grid, kThreads, 0, st>>>(P, wide);
+  }
   prof_after(slot, st);
   return launch_status();
 }
 
 template <typename T>
-int gather_rows(const GatherParams &P, int grid, cudaStream_t st) {
+int gather_rows(GatherParams &P, int grid, cudaStream_t st) {
   constexpr int kV = 16 / (int)sizeof(T);
   const int es = (int)sizeof(T);
   const bool out_wide = paged::rows_aligned(P.out[0], es, 16) && paged::rows_aligned(P.out[1], es, 16);
   const int slot = prof_before(st);
-  if (P.cache.group != 0) gather4_kernel<T><<<grid, kThreads, 0, st>>>(P, out_wide);
-  else if (out_wide && P.cache.head_dim % kV == 0 && paged::cache_aligned(P.cache, es, 16))
+  if (P.cache.group != 0) {
+    if (P.cache.head_dim == 128) gather4_kernel<T, 128><<<grid, kThreads, 0, st>>>(P, out_wide);
+    else gather4_kernel<T, 64><<<grid, kThreads, 0, st>>>(P, out_wide);
+  } else if (out_wide && P.cache.head_dim % kV == 0 && paged::cache_aligned(P.cache, es, 16)) {
+    P.by_lanes = reciprocal(P.cache.head_dim / kV);
     gather_kernel<T, kV><<<grid, kThreads, 0, st>>>(P);
-  else gather_kernel<T, 1><<<grid, kThreads, 0, st>>>(P);
+  } else {
+    P.by_lanes = reciprocal(P.cache.head_dim);
+    gather_kernel<T, 1><<<grid, kThreads, 0, st>>>(P);
+  }
   prof_after(slot, st);
   return launch_status();
 }
@@ -459,7 +575,10 @@ extern "C" SB_API int sb_paged_append(const sb_paged_cache *cache, const sb_page
   P.err = reinterpret_cast<unsigned long long *>(err_counter);
   P.n_q_heads = query.data ? n_q_heads : 0;
   P.rows = 2 * cache->n_heads + P.n_q_heads;
-  P.tokens_per_cta = tokens_per_cta(batch->n_tokens);
+  P.by_rows = reciprocal(P.rows), P.by_lanes = 0;
+  P.plan = row_plan(kThreads / std::max(1, cache->head_dim / (2 * kPer)), P.rows);
+  P.page_shift = page_shift(cache->block_size), P.group_shift = page_shift(cache->group);
+  P.tokens_per_cta = tokens_per_cta(batch->n_tokens, cache->group != 0);
   const int grid = (batch->n_tokens + P.tokens_per_cta - 1) / P.tokens_per_cta;
   const bool neox = rotary_style == SB_ROTARY_NEOX;
   const bool codes = cache->group != 0;
@@ -487,7 +606,10 @@ extern "C" SB_API int sb_paged_gather(const sb_paged_cache *cache, const sb_page
   P.cache = *cache, P.batch = *batch;
   P.out[0] = key_out, P.out[1] = value_out;
   P.err = reinterpret_cast<unsigned long long *>(err_counter);
-  P.tokens_per_cta = tokens_per_cta(batch->n_tokens);
+  P.by_rows = reciprocal(2 * cache->n_heads), P.by_lanes = 0;
+  P.plan = row_plan(kThreads / std::max(1, cache->head_dim / 8), 2 * cache->n_heads);
+  P.page_shift = page_shift(cache->block_size), P.group_shift = page_shift(cache->group);
+  P.tokens_per_cta = tokens_per_cta(batch->n_tokens, cache->group != 0);
   const int grid = (batch->n_tokens + P.tokens_per_cta - 1) / P.tokens_per_cta;
   switch (dtype) {
     case SB_DTYPE_F32: return gather_rows<float>(P, grid, st);

@@ -904,9 +904,7 @@ int launch_decode(const AttendParams &A, int dtype, void *workspace, cudaStream_
   P.heads_per_tile = std::min(A.G, rows);
   P.tokens_per_tile = rows / P.heads_per_tile;
   P.head_tiles = (A.G + P.heads_per_tile - 1) / P.heads_per_tile;
-  P.page_shift = -1;
-  for (int i = 0; i < 31; ++i)
-    if (A.cache.block_size == 1 << i) P.page_shift = i;
+  P.page_shift = page_shift(A.cache.block_size);
   // Short contexts are not worth a second launch: up to 16 blocks of 64 keys a tile are left whole.
   const int64_t held = (int64_t)A.batch.max_blocks * A.cache.block_size;
   const int64_t seen = P.tokens_per_tile == 1 && A.window < 0x7fffffff ? std::min(held, (int64_t)A.window + A.sinks) : held;

@@ -27,7 +27,6 @@ there.
 from __future__ import annotations
 
 import math
-from contextlib import nullcontext
 
 import torch
 
@@ -40,6 +39,8 @@ _freqs: dict[tuple, torch.Tensor] = {}
 
 
 def _need(t, name: str, device: torch.device | None = None) -> None:
+    if isinstance(t, torch.Tensor) and t.is_cuda and (device is None or t.device == device):
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     _lib.require_cuda(t, name)
@@ -47,12 +48,8 @@ def _need(t, name: str, device: torch.device | None = None) -> None:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
-_HERE = nullcontext()
-
-
-def _on(device: torch.device):
-    """The device's context, entered only where it is not the current one."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+# the current device's index, without torch.cuda's initialisation check (the tensors at hand have passed it)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _inv_freq64(rope_base: float, head_dim: int, device: torch.device) -> torch.Tensor:
@@ -213,6 +210,17 @@ def _written(t: torch.Tensor, name: str) -> None:
 _NO_ROWS = _lib.SbTokenRows()
 
 
+def _call(device: torch.device, what: str, fn, *args) -> None:
+    """``fn(*args, stream)`` on the device's current stream, with that device the current one."""
+    if device.index == _current_device():
+        status = fn(*args, _lib.stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _lib.stream_ptr(device))
+    if status:
+        _lib.check(status, what)
+
+
 def append_paged_kv(
     kv_cache: torch.Tensor | Int4KVCache,
     key: torch.Tensor,
@@ -261,12 +269,8 @@ def append_paged_kv(
     style = _rows.rotary_code(rotary_style)
     dev = batch.device
     freq = None if rope_base is None else _inv_freq64(rope_base, hd, dev).data_ptr()
-    with _on(dev):
-        _lib.check(
-            _lib.load().sb_paged_append(c, batch._c, k, v, q, qo, hq, code, freq, style,
-                                        _lib.err_counter(dev).data_ptr(), _lib.stream_ptr(dev)),
-            "append_paged_kv",
-        )
+    _call(dev, "append_paged_kv", _lib.load().sb_paged_append, c, batch._c, k, v, q, qo, hq, code, freq, style,
+          _lib.err_counter(dev).data_ptr())
     return kv_cache
 
 
@@ -304,11 +308,7 @@ def gather_paged_kv(
             raise ValueError(f"out must be [2, {c.n_heads}, {batch._c.n_tokens}, {c.head_dim}], got {tuple(out.shape)}")
         _written(out, "out")
     k, v = (_token_rows(out[i].transpose(0, 1), "out", batch, c.n_heads, c.head_dim, dtype) for i in (0, 1))
-    with _on(dev):
-        _lib.check(
-            _lib.load().sb_paged_gather(c, batch._c, k, v, code, _lib.err_counter(dev).data_ptr(), _lib.stream_ptr(dev)),
-            "gather_paged_kv",
-        )
+    _call(dev, "gather_paged_kv", _lib.load().sb_paged_gather, c, batch._c, k, v, code, _lib.err_counter(dev).data_ptr())
     return out
 
 
@@ -365,15 +365,10 @@ def paged_attention(
         if status.dtype != torch.int32 or status.numel() < 1:
             raise TypeError("status must be an int32 tensor of one element")
     lib = _lib.load()
-    with _on(dev):
-        nbytes = lib.sb_paged_attention_workspace_bytes(c, batch._c, hq, code)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
-        _lib.check(
-            lib.sb_paged_attention(c, batch._c, q, o, hq, window or 0, sinks, scale, code,
-                                   None if ws is None else ws.data_ptr(), nbytes,
-                                   None if status is None else status.data_ptr(), _lib.stream_ptr(dev)),
-            "paged_attention",
-        )
+    nbytes = lib.sb_paged_attention_workspace_bytes(c, batch._c, hq, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
+    _call(dev, "paged_attention", lib.sb_paged_attention, c, batch._c, q, o, hq, window or 0, sinks, scale, code,
+          None if ws is None else ws.data_ptr(), nbytes, None if status is None else status.data_ptr())
     return out
 
 
