@@ -21,7 +21,7 @@ using paged::find_block;
 using paged::find_request_warp;
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 8;    // tokens of a CTA
+constexpr int kMaxTokens = 4;    // tokens of a CTA
 constexpr int kMaxTokens4 = 16;  // 4-bit: a row is four threads, and a block's share of the work is to fill it
 
 // Where a CTA's tokens go; filled by its first threads.
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(kThreads) gather4_kernel(const GatherParams P,
   }
 }
 
-// Tokens a CTA takes: one while more would leave SMs with a single CTA, up to eight (finding a token's place
+// Tokens a CTA takes: one while more would leave SMs with a single CTA, up to four or sixteen (finding a token's place
 // and angles is then shared by as much of the work as fits the block).
 int tokens_per_cta(int n_tokens, bool codes) {
   return std::min(codes ? kMaxTokens4 : kMaxTokens, std::max(1, n_tokens / (2 * paged::sm_count())));

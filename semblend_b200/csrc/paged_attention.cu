@@ -121,7 +121,7 @@ extern "C" SB_API int64_t sb_paged_attention_workspace_bytes(const sb_paged_cach
   paged::AttendParams P = {};
   P.cache = *cache, P.batch = *batch;
   P.Hq = n_q_heads, P.G = n_q_heads / cache->n_heads;
-  P.scale = 1.f;
+  P.scale = 1.f, P.window = 0x7fffffff;  // a window only makes the call need less
   if (paged::prefill_takes(P, dtype))  // with a scale of 0 the decode path takes the call
     return std::max(paged::decode_workspace_bytes(P), paged::prefill_workspace_bytes(P));
   return paged::decode_takes(P, dtype) ? paged::decode_workspace_bytes(P) : 0;
@@ -154,7 +154,8 @@ extern "C" SB_API int sb_paged_attention(const sb_paged_cache *cache, const sb_p
   if (paged::decode_takes(P, dtype)) {
     const bool prefill = paged::prefill_takes(P, dtype);
     const int64_t need = prefill ? paged::prefill_workspace_bytes(P) : paged::decode_workspace_bytes(P);
-    if (!workspace || workspace_bytes < need || !paged::multiple(workspace, 128)) return SB_ERR_WORKSPACE_TOO_SMALL;
+    if (need > 0 && (!workspace || workspace_bytes < need || !paged::multiple(workspace, 128)))
+      return SB_ERR_WORKSPACE_TOO_SMALL;
     if (prefill) return paged::launch_prefill(P, dtype, status, workspace, st);
     return paged::launch_decode(P, dtype, workspace, st);
   }

@@ -49,7 +49,8 @@ template <int D, int GROUP> struct Ring {
   static constexpr int kWarp = kStages * kStage;
 };
 
-constexpr int kWholeKeys = 1024;  // contexts up to this are not split
+constexpr int kWholeKeys = 1024;  // of a CTA where tiles are not cut
+constexpr int kMaxCluster = 8;
 constexpr int kRowPad = 4;  // floats between rows of the join buffer
 template <int D, int GROUP, int NT> constexpr int ring_bytes() {
   return std::max(kWarps * Ring<D, GROUP>::kWarp, kWarps * 8 * NT * (D + kRowPad) * 4);
@@ -80,7 +81,9 @@ struct DecodeParams {
   float *partials;  // [grid][2][R * (D + 2)]
   int tokens_per_tile, heads_per_tile, head_tiles;
   int page_shift;   // block_size as a power of two, or -1
-  int whole;        // 1: tiles are not cut, the line counts them instead of their blocks
+  // > 0: tiles are not cut, the line counts them instead of their blocks; each is shared by the CTAs of a
+  // cluster of this many
+  int whole;
   int dtype;
 };
 
@@ -93,10 +96,7 @@ __host__ __device__ __forceinline__ int cta_of(int64_t base, int more, int64_t x
   return (int)(x < big ? x / (base + 1) : more + (x - big) / base);
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool take) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool take) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
 template <int N> __device__ __forceinline__ void cp_async_small(uint32_t dst, const void *src, bool take) {
@@ -124,6 +124,18 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
+// The other CTAs of a cluster: a barrier with their shared-memory writes before it, and their copy of a value.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float remote(const float *p, int rank) {
+  uint32_t at;
+  float x;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(tc::smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
+
 // c += A(16 x 16) B(16 x 8), fp32 accumulation.
 template <typename T>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -135,6 +147,37 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// c = A B.
+template <typename T>
+__device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// N words from shared memory at a multiple of 4 N bytes.
+template <int N> struct Words {
+  uint32_t w[N];
+};
+template <int N> __device__ __forceinline__ Words<N> load_words(const uint8_t *p) {
+  Words<N> x;
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    x.w[0] = v.x, x.w[1] = v.y, x.w[2] = v.z, x.w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    x.w[0] = v.x, x.w[1] = v.y;
+  } else {
+    x.w[0] = *reinterpret_cast<const uint32_t *>(p);
+  }
+  return x;
 }
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -198,11 +241,13 @@ __global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_ker
   }
   __syncthreads();
   const int64_t total = prefix[B];
-  const int n_ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, total));
+  // CTA (or cluster) number and how many have work
+  const int cta = P.whole ? blockIdx.x / P.whole : blockIdx.x, rank = P.whole ? blockIdx.x % P.whole : 0;
+  const int n_ctas = (int)max((int64_t)1, min((int64_t)(P.whole ? gridDim.x / P.whole : gridDim.x), total));
   const int64_t base_blocks = total / n_ctas;
   const int more = (int)(total - base_blocks * n_ctas);
-  int64_t cur = cut_at(base_blocks, more, blockIdx.x);
-  const int64_t stop = (int)blockIdx.x < n_ctas ? cut_at(base_blocks, more, blockIdx.x + 1) : cur;
+  int64_t cur = cut_at(base_blocks, more, cta);
+  const int64_t stop = cta < n_ctas ? cut_at(base_blocks, more, cta + 1) : cur;
   const int64_t begin = cur;
   if (cur >= stop) {
     if (tid == 0 && !P.whole) P.cuts[blockIdx.x].n_ctas = 0;
@@ -245,8 +290,9 @@ __global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_ker
       at += span;
       tok += P.tokens_per_tile;
     }
-    const int i0 = P.whole ? 0 : (int)(cur - at);
-    const int i1 = P.whole ? tk.n_blocks : (int)min((int64_t)tk.n_blocks, i0 + (stop - cur));
+    const int i0 = P.whole ? (int)((int64_t)tk.n_blocks * rank / P.whole) : (int)(cur - at);
+    const int i1 = P.whole ? (int)((int64_t)tk.n_blocks * (rank + 1) / P.whole)
+                           : (int)min((int64_t)tk.n_blocks, i0 + (stop - cur));
     const int head0 = g * A.G + ht * P.heads_per_tile;
     const int nheads = min(P.heads_per_tile, A.G - ht * P.heads_per_tile);
     if (cur == begin && tid == 0 && !P.whole) {  // whole tiles leave nothing to join
@@ -360,75 +406,76 @@ __global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_ker
       const int c = lane % kChunks;
       return rr * R::kPitch + (GROUP == 0 ? ((c ^ (rr & 7)) << 4) : (c << 4));
     };
-    const bool whole_pages = P.page_shift >= 0 ? (1 << P.page_shift) >= WK : bs % WK == 0;  // a warp's keys in one page
+    // A warp's 16 rows of a 16-bit cache mostly lie in one page: one lookup.  Else (smaller pages, or 32 rows
+    // of codes) every lane looks its own key's page up and the rows' offsets go round by shuffles.
+    const bool one_page = GROUP == 0 && (P.page_shift >= 0 ? (1 << P.page_shift) >= WK : bs % WK == 0);
     auto page_of = [&](int key) -> int {
       const int lb = P.page_shift >= 0 ? key >> P.page_shift : key / bs;
-      if (lb >= A.batch.max_blocks) return -1;
+      if ((unsigned)lb >= (unsigned)A.batch.max_blocks) return -1;  // (nor a key past 2^31 that wrapped)
       const int64_t e = wide_table ? reinterpret_cast<const int64_t *>(table)[lb] : reinterpret_cast<const int32_t *>(table)[lb];
       return (uint64_t)e < (uint64_t)A.cache.n_blocks ? (int)e : -1;
     };
-    auto in_page = [&](int key) -> int { return P.page_shift >= 0 ? key & ((1 << P.page_shift) - 1) : key % bs; };
-    int next_page = whole_pages ? page_of(block_key(tk, i0, KB) + warp * WK) : -1;
+    const int my_key = warp * WK + (one_page ? 0 : lane);
+    // Places inside a page by this lane's key: the same for every block where the page is at most a warp's
+    // keys (else the block's own place in the page comes on top).
+    const bool by_shift = P.page_shift >= 0;
+    const int in_mask = by_shift ? (1 << P.page_shift) - 1 : 0;
+    const int64_t page_bytes = A.cache.stride_block * kElem, page_scale = A.cache.scale_block * 2;
+    const int64_t lane_row = (lane & in_mask & (WK - 1)) * row_bytes;
+    const int64_t lane_scale = (lane & in_mask & (WK - 1)) * (A.cache.scale_pos * 2), v_scale = A.cache.scale_kv * 2;
+    const bool large_pages = in_mask >= WK;
+    const uint32_t to_lane = ring + piece_at(lane / kChunks);  // codes: rows further on lie at a fixed distance
+    const char *first = kbase - (lane / kChunks) * row_bytes;
+    int next_key = block_key(tk, i0, KB) + my_key;
+    int next_page = page_of(next_key);
     auto issue = [&](int i, int s) {
       if (i < i1) {
-        const int key0 = block_key(tk, i, KB) + warp * WK;
+        const int key = next_key, page = next_page, key0 = key - (one_page ? 0 : lane);
+        // the next page's number is on its way behind this block's work
+        next_key = block_key(tk, i + 1, KB) + my_key;
+        if (i + 1 < i1) next_page = page_of(next_key);
+        const uint32_t bits = __ballot_sync(0xffffffffu, lane < WK && page >= 0 && in_span(tk.span, key0 + lane));
+        if (lane == 0) seen_bits[warp * 8 + s] = bits;
         const uint32_t dst = ring + s * R::kStage;
-        uint32_t bits = kAll;
-        if (whole_pages) {
-          const int page = next_page;
-          // the next page's number is on its way behind this block's work
-          if (i + 1 < i1) next_page = page_of(block_key(tk, i + 1, KB) + warp * WK);
-          const int off = in_page(key0);
-          if (!(page >= 0 && key0 + WK <= tk.span.end && (key0 >= tk.span.first || key0 + WK <= tk.span.sink_end)))
-            bits = __ballot_sync(0xffffffffu, lane < WK && page >= 0 && in_span(tk.span, key0 + lane));
-          const char *src = kbase + (int64_t)max(page, 0) * (A.cache.stride_block * kElem) + off * row_bytes;
-          if (bits == kAll) {
-#pragma unroll
-            for (int it = 0; it < WK / kRowsAt; ++it) {
-              const uint32_t to = dst + piece_at(it * kRowsAt + lane / kChunks);
-              cp_async16(to, src);
-              cp_async16(to + R::kTile, src + v_off);
-              src += kRowsAt * row_bytes;
-            }
-          } else {
-#pragma unroll
-            for (int it = 0; it < WK / kRowsAt; ++it) {
-              const int rr = it * kRowsAt + lane / kChunks;
-              const uint32_t to = dst + piece_at(rr);
-              const bool take = (bits >> rr) & 1;
-              cp_async16_or_zero(to, take ? src : kbase, take);
-              cp_async16_or_zero(to + R::kTile, take ? src + v_off : kbase, take);
-              src += kRowsAt * row_bytes;
-            }
-          }
-          if constexpr (GROUP != 0) {
-            const bool in = (bits >> lane) & 1;
-            const char *from = sbase + 2 * ((int64_t)max(page, 0) * A.cache.scale_block + (off + lane) * A.cache.scale_pos);
-            const uint32_t to = dst + WK * R::kPitch + lane * R::kScale;
-            cp_async_small<R::kScale>(to, in ? from : sbase, in);
-            cp_async_small<R::kScale>(to + R::kTile, in ? from + A.cache.scale_kv * 2 : sbase, in);
-          }
-        } else {
-          int64_t row = 0, srow = 0;  // of the lane's key
-          const bool in = lane < WK && in_span(tk.span, key0 + lane) && key_row(A, b, key0 + lane, row, srow);
-          bits = __ballot_sync(0xffffffffu, in);
+        // a key that no row of the tile sees (or without a page) is not read: zeros
+        if (one_page) {
+          const int in = by_shift ? key & in_mask : key % bs;
+          const char *src = kbase + max(page, 0) * page_bytes + in * row_bytes;
 #pragma unroll
           for (int it = 0; it < WK / kRowsAt; ++it) {
             const int rr = it * kRowsAt + lane / kChunks;
-            const char *src = kbase - (lane / kChunks) * row_bytes + __shfl_sync(0xffffffffu, row, rr) * kElem;
             const uint32_t to = dst + piece_at(rr);
             const bool take = (bits >> rr) & 1;
-            cp_async16_or_zero(to, take ? src : kbase, take);
-            cp_async16_or_zero(to + R::kTile, take ? src + v_off : kbase, take);
+            cp_async16(to, src, take);
+            cp_async16(to + R::kTile, src + v_off, take);
+            src += kRowsAt * row_bytes;
+          }
+        } else {
+          int64_t row = max(page, 0) * page_bytes, scale = GROUP == 0 ? 0 : max(page, 0) * page_scale;
+          if (by_shift) {
+            row += lane_row, scale += lane_scale;
+            if (large_pages) row += (key0 & in_mask) * row_bytes, scale += (key0 & in_mask) * (A.cache.scale_pos * 2);
+          } else {
+            row += (key % bs) * row_bytes, scale += (key % bs) * (A.cache.scale_pos * 2);
+          }
+          const uint32_t at = to_lane + s * R::kStage;
+#pragma unroll
+          for (int it = 0; it < WK / kRowsAt; ++it) {
+            const int rr = it * kRowsAt + lane / kChunks;
+            const char *src = first + __shfl_sync(0xffffffffu, row, rr);
+            const uint32_t to = GROUP == 0 ? dst + piece_at(rr) : at + it * kRowsAt * R::kPitch;
+            const bool take = (bits >> rr) & 1;
+            cp_async16(to, src, take);
+            cp_async16(to + R::kTile, src + v_off, take);
           }
           if constexpr (GROUP != 0) {
-            const char *from = sbase + 2 * srow;
+            const bool take = (bits >> lane) & 1;
+            const char *src = sbase + scale;
             const uint32_t to = dst + WK * R::kPitch + lane * R::kScale;
-            cp_async_small<R::kScale>(to, in ? from : sbase, in);
-            cp_async_small<R::kScale>(to + R::kTile, in ? from + A.cache.scale_kv * 2 : sbase, in);
+            cp_async_small<R::kScale>(to, src, take);
+            cp_async_small<R::kScale>(to + R::kTile, src + v_scale, take);
           }
         }
-        if (lane == 0) seen_bits[warp * 8 + s] = bits;
       }
       cp_commit();
     };
@@ -450,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_ker
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[mt][nt][i] = 0.f;
 
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < R::kStages - 1; ++s) issue(i0 + s, s);
     int stage = 0;
     for (int i = i0; i < i1; ++i) {
@@ -472,51 +519,39 @@ __global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_ker
 #pragma unroll
       for (int j = 0; j < SUB; ++j) {
         if constexpr (GROUP == 0) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) sc[j][nt][x] = 0.f;
           const int mat = lane / 8, krow = (mat & 1) * 8 + (lane & 7);
 #pragma unroll
           for (int ks = 0; ks < MT; ++ks) {
             uint32_t a[4];
             ldsm4(a, kt + krow * R::kPitch + (((2 * ks + (mat >> 1)) ^ (krow & 7)) << 4));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma<M>(sc[j][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              if (ks == 0) mma_first<M>(sc[j][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+              else mma<M>(sc[j][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+            }
           }
         } else {
           // codes enter as fp16 subnormals: code * 2^-24 is the bit pattern `code`, so a mask is the conversion
           constexpr int WPG = GROUP / 32;
           const uint8_t *row0 = kp + (16 * j + r) * R::kPitch, *row1 = row0 + 8 * R::kPitch;
-          float2 s0[NG], s1[NG];
+          const Words<NG> k0 = load_words<NG>(kp + WK * R::kPitch + (16 * j + r) * R::kScale);
+          const Words<NG> k1 = load_words<NG>(kp + WK * R::kPitch + (16 * j + r + 8) * R::kScale);
 #pragma unroll
           for (int gq = 0; gq < NG; ++gq) {
-            s0[gq] = unpack_half2(*reinterpret_cast<const uint32_t *>(kp + WK * R::kPitch + (16 * j + r) * R::kScale + 4 * gq));
-            s1[gq] = unpack_half2(*reinterpret_cast<const uint32_t *>(kp + WK * R::kPitch + (16 * j + r + 8) * R::kScale + 4 * gq));
-          }
-#pragma unroll
-          for (int gq = 0; gq < NG; ++gq) {
+            const float2 s0 = unpack_half2(k0.w[gq]), s1 = unpack_half2(k1.w[gq]);
             float dot[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int x = 0; x < 4; ++x) dot[nt][x] = 0.f;
-            uint32_t w0[WPG], w1[WPG];
             const int at_word = 4 * (gq * (GROUP / 8) + q4 * WPG);
+            const Words<WPG> w0 = load_words<WPG>(row0 + at_word), w1 = load_words<WPG>(row1 + at_word);
 #pragma unroll
             for (int e = 0; e < WPG; ++e) {
-              w0[e] = *reinterpret_cast<const uint32_t *>(row0 + at_word + 4 * e);
-              w1[e] = *reinterpret_cast<const uint32_t *>(row1 + at_word + 4 * e);
-            }
-#pragma unroll
-            for (int e = 0; e < WPG; ++e) {
-              const uint32_t x0 = w0[e] >> 8, x1 = w1[e] >> 8;
-              const uint32_t a[4] = {w0[e] & 0x000F000Fu, w1[e] & 0x000F000Fu, w0[e] & 0x00F000F0u, w1[e] & 0x00F000F0u};
+              const uint32_t y0 = w0.w[e], y1 = w1.w[e], x0 = y0 >> 8, x1 = y1 >> 8;
+              const uint32_t a[4] = {y0 & 0x000F000Fu, y1 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x00F000F0u};
               const uint32_t c[4] = {x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u};
               const int wd = gq * WPG + e;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                mma<M>(dot[nt], a, qf[nt][2 * wd][0], qf[nt][2 * wd][1]);
+                if (e == 0) mma_first<M>(dot[nt], a, qf[nt][2 * wd][0], qf[nt][2 * wd][1]);
+                else mma<M>(dot[nt], a, qf[nt][2 * wd][0], qf[nt][2 * wd][1]);
                 mma<M>(dot[nt], c, qf[nt][2 * wd + 1][0], qf[nt][2 * wd + 1][1]);
               }
             }
@@ -524,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_ker
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int x = 0; x < 4; ++x) {
-                const float2 sz = x < 2 ? s0[gq] : s1[gq];
+                const float2 sz = x < 2 ? s0 : s1;
                 const float z = gq == 0 ? sz.y * qsum[nt][x & 1][gq] : fmaf(sz.y, qsum[nt][x & 1][gq], sc[j][nt][x]);
                 sc[j][nt][x] = fmaf(sz.x, dot[nt][x], z);
               }
@@ -538,6 +573,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_ker
 #pragma unroll
           for (int x = 0; x < 4; ++x) sc[j][nt][x] *= row_scale[nt][x & 1];
       if (!all_seen) {
+        __syncwarp();  // a real branch: predicated, the masks would be issued for every block
 #pragma unroll
         for (int j = 0; j < SUB; ++j)
 #pragma unroll
@@ -616,10 +652,11 @@ __global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_ker
           // rounding, but above an fp16 one's, for which what was dropped enters as a second product.
           uint32_t pb[NT][NG][2], pl[NT][NG][2];
           constexpr bool fine = std::is_same<T, __half>::value;
+          const Words<NG> v0s = load_words<NG>(vp + WK * R::kPitch + (16 * j + r) * R::kScale);
+          const Words<NG> v1s = load_words<NG>(vp + WK * R::kPitch + (16 * j + r + 8) * R::kScale);
 #pragma unroll
           for (int gq = 0; gq < NG; ++gq) {
-            const float2 s0 = unpack_half2(*reinterpret_cast<const uint32_t *>(vp + WK * R::kPitch + (16 * j + r) * R::kScale + 4 * gq));
-            const float2 s1 = unpack_half2(*reinterpret_cast<const uint32_t *>(vp + WK * R::kPitch + (16 * j + r + 8) * R::kScale + 4 * gq));
+            const float2 s0 = unpack_half2(v0s.w[gq]), s1 = unpack_half2(v1s.w[gq]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -736,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_ker
           }
       }
     __syncthreads();
-    const bool whole = i0 == 0 && i1 == tk.n_blocks;
+    const bool whole = i0 == 0 && i1 == tk.n_blocks, shared = P.whole > 1;
     float *part = P.partials + ((int64_t)blockIdx.x * 2 + (cur != begin)) * kRows * (D + 2);
     for (int row = warp; row < kRows; row += kWarps) {
       int t, h;
@@ -773,7 +810,14 @@ __global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_ker
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) acc[i] = sums.acc[i];
       }
-      if (whole) {
+      if (shared) {
+        // left in shared memory for the CTA of the cluster that takes this row (this warp alone has read it)
+        float *to = buf + row * (D + kRowPad);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) to[lane + 32 * i] = acc[i];
+        __syncwarp();
+        if (lane == 0) stat_m[row] = m, stat_l[row] = l;
+      } else if (whole) {
         // l is 0 only if no key is seen (a NaN score makes it NaN)
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -786,6 +830,30 @@ __global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_ker
         if (lane == 0) part[kRows * D + row] = m, part[kRows * D + kRows + row] = l;
       }
     }
+    if (shared) {
+      cluster_sync();
+      for (int row = warp; row < kRows; row += kWarps) {
+        int t, h;
+        if (row % P.whole != rank || !row_place(row, t, h)) continue;
+        float m = -INFINITY, l = 0.f, acc[D / 32];
+        for (int k = 0; k < P.whole; ++k) m = fmaxf(m, remote(&stat_m[row], k));
+        const float base = m > -INFINITY ? m : 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+        for (int k = 0; k < P.whole; ++k) {
+          const float w = tc::ex2_approx(remote(&stat_m[row], k) - base);
+          l = fmaf(w, remote(&stat_l[row], k), l);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(w, remote(buf + row * (D + kRowPad) + lane + 32 * i, k), acc[i]);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+          store_any(A.out.data, (int64_t)t * A.out.stride_token + (int64_t)h * A.out.stride_head + lane + 32 * i,
+                    acc[i] * inv, P.dtype);
+      }
+      cluster_sync();  // nobody reads this CTA's rows any more
+    }
     cur += P.whole ? 1 : i1 - i0;
     __syncthreads();  // the join buffer becomes the ring again
   }
@@ -795,41 +863,56 @@ __global__ void __launch_bounds__(kThreads, resident<D, GROUP, NT>()) decode_ker
 // k's range starts in if k is the first to start inside it; the pieces lie in
 // the second slot of CTA k - 1 (its first, if its range starts with the tile)
 // and the first slots of k, k + 1, ...
+// A CTA takes one row (blockIdx.y); its warps take every so many-th piece (a
+// long context alone on the GPU leaves over a hundred, which one CTA per tile
+// took 20 us to read) and add up in shared memory.
+constexpr int kJoinWarps = 2, kJoinThreads = 32 * kJoinWarps;
 template <int D>
-__global__ void __launch_bounds__(256) join_kernel(const DecodeParams P, int rows) {
-  const int k = blockIdx.x;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeParams P, int rows) {
+  __shared__ float sums[kJoinWarps][D + 1];
+  const int k = blockIdx.x, row = blockIdx.y;
   const CutUnit c = P.cuts[k];
   if (k == 0 || k >= c.n_ctas) return;
   const int64_t mine = cut_at(c.base, c.more, k), before = cut_at(c.base, c.more, k - 1);
   if (mine == c.start || before > c.start) return;
   const int last = cta_of(c.base, c.more, c.end - 1);
-  const int lane = threadIdx.x % 32;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int pi = row / P.heads_per_tile, hh = row - pi * P.heads_per_tile;
+  if (pi >= c.n_tok || hh >= c.n_heads) return;
   const int64_t slot = (int64_t)rows * (D + 2);
   const float *first = P.partials + ((int64_t)(k - 1) * 2 + (before != c.start)) * slot;
-  for (int row = threadIdx.x / 32; row < rows; row += blockDim.x / 32) {
-    const int pi = row / P.heads_per_tile, hh = row - pi * P.heads_per_tile;
-    if (pi >= c.n_tok || hh >= c.n_heads) continue;
-    float m = -INFINITY;
-    for (int j = k - 1 + lane; j <= last; j += 32)
-      m = fmaxf(m, (j < k ? first : P.partials + (int64_t)j * 2 * slot)[rows * D + row]);
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m > -INFINITY ? m : 0.f;
-    float l = 0.f, acc[D / 32];
+  const float *others = P.partials + (int64_t)k * 2 * slot;  // pieces of k, k + 1, ...: two slots apart
+  const int pieces = last - k + 2;
+  float m = -INFINITY;
+  for (int j = lane; j < pieces; j += 32)
+    m = fmaxf(m, (j == 0 ? first : others + (int64_t)(j - 1) * 2 * slot)[rows * D + row]);
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float base = m > -INFINITY ? m : 0.f;
+  float l = 0.f, acc[D / 32];
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-#pragma unroll 4
-    for (int j = k - 1; j <= last; ++j) {
-      const float *part = j < k ? first : P.partials + (int64_t)j * 2 * slot;
-      const float w = tc::ex2_approx(part[rows * D + row] - base);
-      l = fmaf(w, part[rows * D + rows + row], l);
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+#pragma unroll 8
+  for (int j = warp; j < pieces; j += kJoinWarps) {
+    const float *part = j == 0 ? first : others + (int64_t)(j - 1) * 2 * slot;
+    const float w = tc::ex2_approx(part[rows * D + row] - base);
+    l = fmaf(w, part[rows * D + rows + row], l);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(w, part[row * D + lane + 32 * i], acc[i]);
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int64_t at = (int64_t)(c.tok + pi) * P.a.out.stride_token + (int64_t)(c.head + hh) * P.a.out.stride_head;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) store_any(P.a.out.data, at + lane + 32 * i, acc[i] * inv, P.dtype);
+    for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(w, part[row * D + lane + 32 * i], acc[i]);
   }
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) sums[warp][lane + 32 * i] = acc[i];
+  if (lane == 0) sums[warp][D] = l;
+  __syncthreads();
+  if (warp != 0) return;
+  for (int w = 1; w < min(kJoinWarps, pieces); ++w) {
+    l += sums[w][D];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] += sums[w][lane + 32 * i];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t at = (int64_t)(c.tok + pi) * P.a.out.stride_token + (int64_t)(c.head + hh) * P.a.out.stride_head;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) store_any(P.a.out.data, at + lane + 32 * i, acc[i] * inv, P.dtype);
 }
 
 // Rows of a tile: eight where a request's rows fit them, else sixteen.
@@ -857,13 +940,25 @@ int run(const DecodeParams &P, cudaStream_t st) {
   constexpr int kSmem = smem_bytes<D, GROUP, NT>();
   static_assert(kSmem <= 227 * 1024, "shared memory");
   if (ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), kSmem) != SB_OK) return SB_ERR_CUDA;
-  const int grid = P.whole ? (int)std::min<int64_t>(max_tiles(P), 1 << 20) : max_grid(P.a, resident<D, GROUP, NT>());
+  const int grid = P.whole ? (int)std::min<int64_t>(max_tiles(P), 1 << 20) * P.whole
+                           : max_grid(P.a, resident<D, GROUP, NT>());
   const int slot = prof_before(st);
-  kernel<<<grid, kThreads, kSmem, st>>>(P);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = kSmem, cfg.stream = st;
+  cudaLaunchAttribute cluster[1];
+  cluster[0].id = cudaLaunchAttributeClusterDimension;
+  cluster[0].val.clusterDim.x = P.whole > 1 ? P.whole : 1;
+  cluster[0].val.clusterDim.y = cluster[0].val.clusterDim.z = 1;
+  cfg.attrs = cluster, cfg.numAttrs = P.whole > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P);
   prof_after(slot, st);
   int s = launch_status();
+  if (e != cudaSuccess) {
+    set_last_cuda_error(e);
+    return SB_ERR_CUDA;
+  }
   if (s != SB_OK || grid == 1 || P.whole) return s;
-  join_kernel<D><<<grid, 256, 0, st>>>(P, 8 * NT);
+  join_kernel<D><<<dim3(grid, 8 * NT), kJoinThreads, 0, st>>>(P, 8 * NT);
   return launch_status();
 }
 
@@ -889,26 +984,42 @@ bool decode_takes(const AttendParams &P, int dtype) {
          multiple(P.cache.scale_head * 2, sb) && multiple(P.cache.scale_pos * 2, sb);
 }
 
-int64_t decode_workspace_bytes(const AttendParams &P) {
-  const int64_t grid = max_grid(P, kMaxResident);
-  return ((grid * (int64_t)sizeof(CutUnit) + 15) / 16) * 16 + grid * 2 * 16 * (P.cache.head_dim + 2) * 4;
-}
-
-int launch_decode(const AttendParams &A, int dtype, void *workspace, cudaStream_t st) {
+namespace {
+DecodeParams plan(const AttendParams &A, int dtype) {
   DecodeParams P;
-  P.dtype = dtype;
+  P.a = A, P.dtype = dtype;
   const int rows = tile_rows(A);
-  const int64_t cut_bytes = ((int64_t)max_grid(A, kMaxResident) * (int64_t)sizeof(CutUnit) + 15) / 16 * 16;
-  P.cuts = reinterpret_cast<CutUnit *>(workspace);
-  P.partials = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + cut_bytes);
+  P.cuts = nullptr, P.partials = nullptr;
   P.heads_per_tile = std::min(A.G, rows);
   P.tokens_per_tile = rows / P.heads_per_tile;
   P.head_tiles = (A.G + P.heads_per_tile - 1) / P.heads_per_tile;
   P.page_shift = page_shift(A.cache.block_size);
-  // Short contexts are not worth a second launch: up to 16 blocks of 64 keys a tile are left whole.
+  // Short contexts are not worth cutting and a second launch: a cluster of up to eight CTAs, as many as the
+  // GPU has room for with all tiles and have 128 keys each, takes a tile whole, as long as that leaves a CTA
+  // at most kWholeKeys.  (One request of 517 keys, 28/4 heads: one CTA a tile 13.2 us, cut 11.4, eight 9.2; of
+  // 4,000: cut 16.8, eight 14.9; of 8,000 both 22.)
   const int64_t held = (int64_t)A.batch.max_blocks * A.cache.block_size;
   const int64_t seen = P.tokens_per_tile == 1 && A.window < 0x7fffffff ? std::min(held, (int64_t)A.window + A.sinks) : held;
-  P.whole = seen <= kWholeKeys;
+  int cluster = 1;
+  while (cluster < kMaxCluster && max_tiles(P) * cluster * 2 <= 2 * sm_count() && seen > 128 * cluster) cluster *= 2;
+  P.whole = seen <= (int64_t)kWholeKeys * cluster ? cluster : 0;
+  return P;
+}
+int64_t cut_bytes(const AttendParams &A) {
+  return ((int64_t)max_grid(A, kMaxResident) * (int64_t)sizeof(CutUnit) + 15) / 16 * 16;
+}
+}  // namespace
+
+int64_t decode_workspace_bytes(const AttendParams &P) {
+  if (plan(P, SB_DTYPE_BF16).whole) return 0;
+  return cut_bytes(P) + (int64_t)max_grid(P, kMaxResident) * 2 * 16 * (P.cache.head_dim + 2) * 4;
+}
+
+int launch_decode(const AttendParams &A, int dtype, void *workspace, cudaStream_t st) {
+  DecodeParams P = plan(A, dtype);
+  const int rows = tile_rows(A);
+  P.cuts = reinterpret_cast<CutUnit *>(workspace);
+  P.partials = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + cut_bytes(A));
   // a launch takes at most kMaxRequests requests; later ones of the stream reuse the workspace
   for (int b = 0; b < A.batch.batch; b += kMaxRequests) {
     P.a = A;
