@@ -36,6 +36,9 @@ INT4_GROUPS = (32, 64, 128)
 INT4_HEAD_DIMS = (64, 128)
 
 _freqs: dict[tuple, torch.Tensor] = {}
+# a cache's description but for its addresses, by shapes, strides, type and layout: every layer of every step asks
+# for the same one
+_geometry: dict[tuple, _lib.SbPagedCache] = {}
 
 
 def _need(t, name: str, device: torch.device | None = None) -> None:
@@ -76,7 +79,7 @@ class PagedBatch:
     what they then hold.
     """
 
-    __slots__ = ("block_tables", "cu_seqlens", "positions", "device", "_c")
+    __slots__ = ("block_tables", "cu_seqlens", "positions", "device", "n_tokens", "_c")
 
     def __init__(self, block_tables: torch.Tensor, cu_seqlens: torch.Tensor, positions: torch.Tensor):
         _need(block_tables, "block_tables")
@@ -98,13 +101,10 @@ class PagedBatch:
         if positions.ndim != 1 or not positions.is_contiguous():
             raise ValueError(f"positions must be a contiguous 1-D tensor, got {tuple(positions.shape)}")
         self.block_tables, self.cu_seqlens, self.positions, self.device = block_tables, cu_seqlens, positions, dev
+        self.n_tokens = positions.shape[0]
         self._c = _lib.SbPagedBatch(block_tables.data_ptr(), cu_seqlens.data_ptr(), positions.data_ptr(), row, batch,
                                     positions.shape[0], max_blocks, _lib.index_code(block_tables.dtype),
                                     _lib.index_code(positions.dtype), 0)
-
-    @property
-    def n_tokens(self) -> int:
-        return self._c.n_tokens
 
 
 class Int4KVCache:
@@ -124,22 +124,36 @@ class Int4KVCache:
         _need(scales, "scales", codes.device)
         if codes.dtype != torch.uint8 or scales.dtype != torch.float16:
             raise TypeError(f"codes must be uint8 and scales float16, got {codes.dtype} and {scales.dtype}")
+        key = (codes.shape, codes.stride(), scales.shape, scales.stride(), layout)
+        known = _geometry.get(key)
+        if known is None:
+            known = self._describe(codes, scales, layout)
+            if len(_geometry) >= 1024:
+                _geometry.clear()
+            _geometry[key] = known
+        self.codes, self.scales, self.layout, self.device = codes, scales, layout, codes.device
+        self._c = c = _lib.SbPagedCache.from_buffer_copy(known)
+        c.data, c.scales = codes.data_ptr(), scales.data_ptr()
+        self.head_dim, self.group = c.head_dim, c.group
+
+    @staticmethod
+    def _describe(codes: torch.Tensor, scales: torch.Tensor, layout: str) -> _lib.SbPagedCache:
         if layout not in _rows.LAYOUTS:
             raise ValueError(f"unknown KV layout {layout!r}; expected one of {_rows.LAYOUTS}")
         nb, nh, bs, half = _rows.paged_geometry(codes.shape, layout)
         if scales.ndim != 6 or scales.shape[:4] != codes.shape[:4] or scales.shape[5] != 2 or scales.shape[4] < 1:
             raise ValueError(f"scales {tuple(scales.shape)} do not match codes {tuple(codes.shape)}")
-        self.codes, self.scales, self.layout, self.device = codes, scales, layout, codes.device
-        self.head_dim, self.group = 2 * half, 2 * half // scales.shape[4]
-        if self.head_dim not in INT4_HEAD_DIMS or self.group not in INT4_GROUPS or self.group * scales.shape[4] != self.head_dim:
+        head_dim, groups = 2 * half, scales.shape[4]
+        group = head_dim // groups
+        if head_dim not in INT4_HEAD_DIMS or group not in INT4_GROUPS or group * groups != head_dim:
             raise ValueError(
-                f"a 4-bit cache holds rows of {INT4_HEAD_DIMS} elements in groups of {INT4_GROUPS}; got {self.head_dim} "
-                f"elements in {scales.shape[4]} groups"
+                f"a 4-bit cache holds rows of {INT4_HEAD_DIMS} elements in groups of {INT4_GROUPS}; got {head_dim} "
+                f"elements in {groups} groups"
             )
-        if codes.stride(4) != 1 or scales.stride(5) != 1 or (scales.shape[4] > 1 and scales.stride(4) != 2):
+        if codes.stride(4) != 1 or scales.stride(5) != 1 or (groups > 1 and scales.stride(4) != 2):
             raise ValueError("the rows of codes and scales must be contiguous")
-        self._c = _lib.SbPagedCache(codes.data_ptr(), scales.data_ptr(), *_axis_strides(codes, layout),
-                                    *_axis_strides(scales, layout), nb, bs, nh, self.head_dim, self.group, 0)
+        return _lib.SbPagedCache(None, None, *_axis_strides(codes, layout), *_axis_strides(scales, layout), nb, bs, nh,
+                                 head_dim, group, 0)
 
     @classmethod
     def allocate(cls, num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int, *, group: int = 64,
@@ -178,19 +192,28 @@ def _cache(kv_cache, batch: PagedBatch, layout: str) -> _lib.SbPagedCache:
             raise ValueError(f"kv_cache is on {kv_cache.device}, expected {batch.device}")
         return kv_cache._c
     _need(kv_cache, "kv_cache", batch.device)
-    layout = _rows.resolve_layout(kv_cache, layout)
-    nb, nh, bs, hd = _rows.paged_geometry(kv_cache.shape, layout)
-    if hd > 1 and kv_cache.stride(4) != 1:
-        raise ValueError("the rows of kv_cache must be contiguous")
-    return _lib.SbPagedCache(kv_cache.data_ptr(), None, *_axis_strides(kv_cache, layout), 0, 0, 0, 0, nb, bs, nh, hd, 0,
-                             _lib.dtype_code(kv_cache.dtype))
+    key = (kv_cache.shape, kv_cache.stride(), kv_cache.dtype, layout)
+    known = _geometry.get(key)
+    if known is None:
+        layout = _rows.resolve_layout(kv_cache, layout)
+        nb, nh, bs, hd = _rows.paged_geometry(kv_cache.shape, layout)
+        if hd > 1 and kv_cache.stride(4) != 1:
+            raise ValueError("the rows of kv_cache must be contiguous")
+        known = _lib.SbPagedCache(None, None, *_axis_strides(kv_cache, layout), 0, 0, 0, 0, nb, bs, nh, hd, 0,
+                                  _lib.dtype_code(kv_cache.dtype))
+        if len(_geometry) >= 1024:
+            _geometry.clear()
+        _geometry[key] = known
+    c = _lib.SbPagedCache.from_buffer_copy(known)
+    c.data = kv_cache.data_ptr()
+    return c
 
 
 def _token_rows(t: torch.Tensor, name: str, batch: PagedBatch, heads: int | None, head_dim: int,
                 dtype: torch.dtype) -> _lib.SbTokenRows:
     """A ``[T, heads, D]`` tensor with contiguous rows."""
     _need(t, name, batch.device)
-    n = batch._c.n_tokens
+    n = batch.n_tokens
     if t.ndim != 3 or t.shape != (n, t.shape[1] if heads is None else heads, head_dim):
         raise ValueError(f"{name} must be [{n}, {'heads' if heads is None else heads}, {head_dim}], got {tuple(t.shape)}")
     if t.dtype != dtype:
@@ -250,11 +273,11 @@ def append_paged_kv(
     c = _cache(kv_cache, batch, layout)
     dtype = key.dtype if isinstance(kv_cache, Int4KVCache) else kv_cache.dtype
     code = _lib.dtype_code(dtype)
-    hd = c.head_dim
+    hd, nh = c.head_dim, c.n_heads
     if hd % 2 or hd > 512:
         raise ValueError(f"head_dim must be even and at most 512, got {hd}")
-    k = _token_rows(key, "key", batch, c.n_heads, hd, dtype)
-    v = _token_rows(value, "value", batch, c.n_heads, hd, dtype)
+    k = _token_rows(key, "key", batch, nh, hd, dtype)
+    v = _token_rows(value, "value", batch, nh, hd, dtype)
     if (query is None) != (query_out is None):
         raise ValueError("query and query_out come together")
     q = qo = _NO_ROWS
@@ -301,11 +324,11 @@ def gather_paged_kv(
     code = _lib.dtype_code(dtype)
     dev = batch.device
     if out is None:
-        out = torch.zeros(2, c.n_heads, batch._c.n_tokens, c.head_dim, dtype=dtype, device=dev)
+        out = torch.zeros(2, c.n_heads, batch.n_tokens, c.head_dim, dtype=dtype, device=dev)
     else:
         _need(out, "out", dev)
         if out.ndim != 4 or out.shape[0] != 2:
-            raise ValueError(f"out must be [2, {c.n_heads}, {batch._c.n_tokens}, {c.head_dim}], got {tuple(out.shape)}")
+            raise ValueError(f"out must be [2, {c.n_heads}, {batch.n_tokens}, {c.head_dim}], got {tuple(out.shape)}")
         _written(out, "out")
     k, v = (_token_rows(out[i].transpose(0, 1), "out", batch, c.n_heads, c.head_dim, dtype) for i in (0, 1))
     _call(dev, "gather_paged_kv", _lib.load().sb_paged_gather, c, batch._c, k, v, code, _lib.err_counter(dev).data_ptr())
