@@ -490,8 +490,8 @@ typedef struct sb_token_rows {
  * in fp32, one rounding to `dtype`, which is the cache's.  4-bit caches: K is
  * rotated in 64 bits and rounded to fp32 (so that codes do not depend on the
  * last bits of cos and sin); per group, with min and max limited to +-60000,
- * zero = fp16(min), step = fp16((max - min) / 15), code = the nearest integer
- * to (x - zero) * (1 / step) in fp32, limited to 0..15; a group that holds a
+ * zero = fp16(min), step = fp16((max - min) * fp32(1 / 15)), code = the nearest
+ * integer to (x - zero) * fp32(1 / step), all in fp32, limited to 0..15; a group that holds a
  * NaN reads back as NaN.  A token
  * whose position addresses no row is not written and counted once in
  * *err_counter (device uint64, may be NULL).  No two tokens of a call may

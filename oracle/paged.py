@@ -56,7 +56,7 @@ def quantise(x: torch.Tensor, group: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Codes and (step, zero) of rows rounded to fp32, each operation rounded to fp32."""
     g = x.float().unflatten(-1, (-1, group))
     lo, hi = g.amin(-1).clamp(-60000, 60000), g.amax(-1).clamp(-60000, 60000)
-    zero, step = lo.half(), ((hi - lo) / 15).half()
+    zero, step = lo.half(), ((hi - lo) * torch.tensor(1 / 15, dtype=torch.float32)).half()
     inv = torch.where(step.float() > 0, 1.0 / step.float(), torch.zeros(()))
     codes = ((g - zero.float()[..., None]) * inv[..., None]).round().clamp(0, 15).nan_to_num(0.0)
     return codes.flatten(-2).to(torch.uint8), torch.stack([step, zero], -1)

@@ -257,7 +257,7 @@ __device__ __forceinline__ void extend(float (&lo)[2], float (&hi)[2], int k, fl
 __device__ __forceinline__ __half2 group_scale(float lo, float hi, float &zero, float &inv) {
   lo = saturate(lo), hi = saturate(hi);
   const __half z = __float2half_rn(lo);
-  const __half st = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+  const __half st = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f));
   zero = __half2float(z);
   const float s = __half2float(st);
   inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;

@@ -976,7 +976,7 @@ int by_type(const DecodeParams &P, int rows, cudaStream_t st) {
 
 // 16-bit rows or codes of head_dim 64 or 128 whose rows and queries start at multiples of 16 bytes.
 bool decode_takes(const AttendParams &P, int dtype) {
-  if (dtype == SB_DTYPE_F32 || (P.cache.head_dim != 64 && P.cache.head_dim != 128)) return false;
+  if (dtype == SB_DTYPE_F32 || P.cache.n_blocks == 0 || (P.cache.head_dim != 64 && P.cache.head_dim != 128)) return false;
   if (!rows_aligned(P.q, 2, 16)) return false;
   if (P.cache.group == 0) return cache_aligned(P.cache, 2, 16);
   const int sb = 4 * (P.cache.head_dim / P.cache.group);  // a row's scales are copied in one piece

@@ -943,9 +943,13 @@ int run_codes(PrefillParams &P, int32_t *status, void *workspace, cudaStream_t s
 // Enough rows per request to fill tiles of 128; pages that cut a block of 128 keys evenly, in whole swizzle
 // groups of 8 rows.
 bool prefill_takes(const AttendParams &P, int dtype) {
-  if (!decode_takes(P, dtype) || P.G > kBM || P.scale == 0.f || P.cache.n_blocks == 0 || P.batch.max_blocks == 0)
-    return false;
+  if (!decode_takes(P, dtype) || P.G > kBM || P.scale == 0.f || P.batch.max_blocks == 0) return false;
   if (!rows_aligned(P.out, 2, 16)) return false;
+  // a tensor map wants every stride it uses to be one
+  const sb_paged_cache &c = P.cache;
+  if (c.group == 0 && ((c.block_size > 1 && c.stride_pos == 0) || (c.n_heads > 1 && c.stride_head == 0) ||
+                       (c.n_blocks > 1 && c.stride_block == 0)))
+    return false;
   const int bs = P.cache.block_size;
   if (bs % 8 || (bs < kBN ? kBN % bs : bs % kBN)) return false;
   if (P.cache.group != 0 && (held_keys(P) >= (1ll << 31) || head_bytes(P) > kMaxHeadBytes ||

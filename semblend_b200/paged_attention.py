@@ -17,7 +17,8 @@ All three take either a per-layer cache tensor (float32, float16 or bfloat16,
 in any of the layouts of the inject) or an :class:`Int4KVCache`, which holds
 the same rows in 4 bits with a step and a zero per group of 32, 64 or 128
 elements.  They run on the tensors' device and its current stream, never
-synchronise, and can be captured into a CUDA graph.  There is no CPU path:
+synchronise, and can be captured into a CUDA graph (after a first call with the
+same ``rope_base`` on the device, which uploads its frequencies).  There is no CPU path:
 host tensors raise :class:`~semblend_b200._lib.NativeLibraryError`.
 
 The reference leaves this part to the serving engine, so it has no counterpart
@@ -261,7 +262,9 @@ def append_paged_kv(
     ``key`` / ``value`` are ``[T, H, D]`` before the rotation (any token and
     head strides, so slices of a fused projection do) in the cache's dtype; a
     4-bit cache takes any of the three dtypes and quantises each row by its
-    groups.  ``rope_base=None`` writes K as it is.  With ``query``
+    groups (``zero = fp16(min)``, ``step = fp16((max - min) / 15)``, the nearest
+    of the 16 values; a group with a NaN reads back as NaN, values beyond 60000
+    are limited).  ``rope_base=None`` writes K as it is.  With ``query``
     ``[T, Hq, D]`` its rotated rows are written to ``query_out``, which may be
     ``query`` itself.  Angles are formed in 64 bits, so far positions keep
     their fraction of a turn.  A token whose position lies outside its
@@ -271,7 +274,14 @@ def append_paged_kv(
     returned.
     """
     c = _cache(kv_cache, batch, layout)
-    dtype = key.dtype if isinstance(kv_cache, Int4KVCache) else kv_cache.dtype
+    if isinstance(kv_cache, Int4KVCache):
+        _need(key, "key", batch.device)
+        dtype = key.dtype
+        _written(kv_cache.codes, "kv_cache")
+        _written(kv_cache.scales, "kv_cache")
+    else:
+        dtype = kv_cache.dtype
+        _written(kv_cache, "kv_cache")
     code = _lib.dtype_code(dtype)
     hd, nh = c.head_dim, c.n_heads
     if hd % 2 or hd > 512:
