@@ -67,26 +67,37 @@ struct PrefillParams {
   int Pt;                // tokens of a tile
   int slots;             // unit slots of a KV head: n_tokens / (2 Pt) + batch
   int64_t n_units;
+  // units from `whole` on are cut into pieces of at least kPieceBlocks blocks, at most `splits` of them: a work
+  // item is a unit below `whole`, then a piece
+  int64_t whole, n_items;
+  int splits;
+  float *partials;       // workspace: of each piece 256 rows of D sums, then 256 pairs of maximum and sum
   int pages, page_rows;  // pages of a block of 128 keys and the rows a box takes of one
   int linear;            // 1: rows expanded to the workspace, [request][head - head0][key]
   int head0, heads;      // KV heads of this launch
   int dtype;             // of query and out
   unsigned *next;        // workspace, zeroed ahead of the launch
+  unsigned *odd;         // the same: whether a cut unit's V rows had odd values
   int *status;
 };
 
 // One unit as its roles see it.
 struct Unit {
   int b, g, tok, n0, n1;     // request, KV head, first token, tokens of the two tiles
-  int nblk0, nblk1;          // blocks each tile goes through
+  int j0;                    // first block of the piece
+  int nblk0, nblk1;          // where the blocks each tile goes through end
   int sink_blocks, w0;
   int first, end, sink_end;  // keys some row sees
   int pmin, pmax;            // smallest position (-1: a token that sees nothing) and largest
   int holes;                 // 1: an unmapped page among the keys
   int number;                // of the unit in the call
+  int piece;                 // of the cut units, or -1: a whole one
   int stop;                  // 1: no more units
 };
 constexpr int kUnitInts = sizeof(Unit) / 4;
+constexpr int kPieceRows = 2 * kBM;
+constexpr int kPieceBlocks = 8;  // a piece costs about three blocks besides its own
+template <int D> constexpr int64_t kPieceFloats = (int64_t)kPieceRows * (D + 2);
 constexpr int kOddUnits = 128;  // units a CTA keeps for the pass over odd values; more: it goes through all
 
 __device__ __forceinline__ int unit_block_key(const Unit &u, int i) {
@@ -118,9 +129,28 @@ __device__ __forceinline__ uint32_t pack_any(float a, float b, int dtype) {
   return dtype == SB_DTYPE_BF16 ? Pack2<__nv_bfloat16>::pack(a, b) : Pack2<__half>::pack(a, b);
 }
 
-// Unit u of the call, found by a whole warp (lanes share the scans); false if
-// the slot holds no tokens.
-__device__ __forceinline__ bool make_unit(const PrefillParams &P, unsigned u, Unit &w) {
+// Whether an unmapped page lies among the unit's keys in its blocks, by a whole warp.
+__device__ __forceinline__ void find_holes(const AttendParams &A, Unit &w) {
+  const int lane = threadIdx.x & 31, bs = A.cache.block_size, nb = max(w.nblk0, w.nblk1);
+  bool bad = false;
+  for (int part = 0; part < 2; ++part) {
+    const int64_t shift = part == 0 ? 0 : w.w0 - w.sink_blocks;
+    const int from = part == 0 ? w.j0 : max(w.j0, w.sink_blocks), to = part == 0 ? min(nb, w.sink_blocks) : nb;
+    // (the last sinks may lie in the window's first block)
+    const int low = part == 0 ? 0 : w.sink_end > w.w0 * kBN ? w.w0 * kBN : w.first;
+    const int k0 = (int)max((int64_t)low, (from + shift) * kBN);
+    const int k1 = (int)min((int64_t)(part == 0 ? w.sink_end : w.end), (to + shift) * kBN);
+    if (to <= from || k1 <= k0) continue;
+    const int p1 = (k1 - 1) / bs;
+#pragma unroll 4
+    for (int p = k0 / bs + lane; p <= p1; p += 32) bad |= find_block(A.batch, w.b, p, A.cache.n_blocks) < 0;
+  }
+  w.holes = __any_sync(0xffffffffu, bad);
+}
+
+// Unit u of the call but for its holes, found by a whole warp (lanes share the
+// scans); false if the slot holds no tokens.
+__device__ __forceinline__ bool find_unit(const PrefillParams &P, unsigned u, Unit &w) {
   const AttendParams &A = P.a;
   const int lane = threadIdx.x & 31, two = 2 * P.Pt;
   // later tokens, which see most without a window, first; the KV heads of a slot side by side
@@ -165,17 +195,29 @@ __device__ __forceinline__ bool make_unit(const PrefillParams &P, unsigned u, Un
   // every tile goes through the blocks from the unit's first on; one that sees nothing through one block
   w.nblk0 = max(1, w.sink_blocks + max(0, (int)(((int64_t)e0 + kBN - 1) / kBN) - w.w0));
   w.nblk1 = w.n1 > 0 ? max(1, w.sink_blocks + max(0, (int)(((int64_t)e1 + kBN - 1) / kBN) - w.w0)) : 0;
+  w.j0 = 0, w.piece = -1;
   w.stop = 0;
-  const int bs = A.cache.block_size;
-  bool bad = false;
-  for (int part = 0; part < 2; ++part) {
-    const int k0 = part == 0 ? 0 : w.first, k1 = part == 0 ? w.sink_end : w.end;
-    if (k1 <= k0) continue;
-    const int p1 = (k1 - 1) / bs;
-#pragma unroll 4
-    for (int p = k0 / bs + lane; p <= p1; p += 32) bad |= find_block(A.batch, w.b, p, A.cache.n_blocks) < 0;
+  return true;
+}
+
+// Blocks of a piece of a unit of nb blocks.
+__device__ __forceinline__ int piece_blocks(const PrefillParams &P, int nb) {
+  return max(kPieceBlocks, (nb + P.splits - 1) / P.splits);
+}
+
+// Work item `item` of the call, by a whole warp; false if there is nothing to do.
+__device__ __forceinline__ bool make_item(const PrefillParams &P, unsigned item, Unit &w) {
+  const AttendParams &A = P.a;
+  const unsigned cut = item < P.whole ? 0 : item - (unsigned)P.whole;
+  if (!find_unit(P, item < P.whole ? item : (unsigned)P.whole + cut / P.splits, w)) return false;
+  if (item >= P.whole) {
+    const int nb = max(w.nblk0, w.nblk1), per = piece_blocks(P, nb);
+    const int64_t j0 = (int64_t)(cut % P.splits) * per;
+    if (j0 >= nb) return false;
+    w.piece = (int)cut, w.j0 = (int)j0;
+    w.nblk0 = (int)min((int64_t)w.nblk0, j0 + per), w.nblk1 = (int)min((int64_t)w.nblk1, j0 + per);
   }
-  w.holes = __any_sync(0xffffffffu, bad);
+  find_holes(A, w);
   return true;
 }
 
@@ -329,13 +371,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         unsigned u = 0;
         if (lane == 0) u = atomicAdd(P.next, 1u);
         u = __shfl_sync(0xffffffffu, u, 0);
-        if (u >= P.n_units) {
+        if (u >= P.n_items) {
           memset(&w, 0, sizeof(w));
           w.stop = 1;
           push_unit(w);
           break;
         }
-        if (!make_unit(P, u, w)) continue;
+        if (!make_item(P, u, w)) continue;
         if (!push_unit(w)) break;
         const int nb = max(w.nblk0, w.nblk1);
         // coordinates of this lane's box of block i
@@ -353,8 +395,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           blk = phys < 0 ? A.cache.n_blocks : phys;
         };
         int row = 0, blk = 0;
-        if (mine) place(0, row, blk);
-        for (int j = 0; j < nb; ++j) {
+        if (mine) place(w.j0, row, blk);
+        for (int j = w.j0; j < nb; ++j) {
           const uint32_t st = gl % kStages, ph = (gl / kStages) & 1;
           int row1 = 0, blk1 = 0;
           if (mine && j + 1 < nb) place(j + 1, row1, blk1);
@@ -422,12 +464,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t ks = gl % kStages;
             if (!tc::mbar_wait(&k_full[ks], (gl / kStages) & 1, ab, 3, kWaitCycles)) break;
             tc::fence_after_sync();
-            issue_s(0, ks);
-            if (w.nblk1 > 0) issue_s(1, ks);
+            if (w.nblk0 > w.j0) issue_s(0, ks);
+            if (w.nblk1 > w.j0) issue_s(1, ks);
             tc::mma_commit(&k_empty[ks]);
           }
-          for (int j = 0; j < nb && ok; ++j) {
-            const uint32_t g = gl + j;
+          for (int j = w.j0; j < nb && ok; ++j) {
+            const uint32_t g = gl + (j - w.j0);
             const uint32_t vs = g % kStages, vph = (g / kStages) & 1;
             const uint32_t ks1 = (g + 1) % kStages, kph1 = ((g + 1) / kStages) & 1;
             bool v_ready = false, k_ready = false;
@@ -454,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int kk = 0; kk < kBN / 32; ++kk)
                 tc::mma_bf16_ts(tmem + tmem_o(t), p_tmem + kk * 8, dv + kk * (2048 >> 4), idesc_pv,
-                                (j == 0 && kk == 0) ? 0u : 1u);
+                                (j == w.j0 && kk == 0) ? 0u : 1u);
               if (!tc::mbar_wait(&p_full[2 * t + 1], pc[t] & 1, ab, 3, kWaitCycles)) {
                 ok = false;
                 continue;
@@ -482,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (j + 1 < nb) tc::mma_commit(&k_empty[ks1]);
           }
           if (!ok) break;
-          gl += nb;
+          gl += nb - w.j0;
           tc::mma_commit(q_empty);
           ++qi;
         }
@@ -499,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!pop_unit(n, true, w)) break;
         const int nb = max(w.nblk0, w.nblk1);
         uint32_t found = 0;
-        for (int j = 0; j < nb; ++j, ++gl) {
+        for (int j = w.j0; j < nb; ++j, ++gl) {
           const int key0 = unit_block_key(w, j);
           const uint32_t st = gl % kStages;
           ok = __all_sync(0xffffffffu, tc::mbar_wait(&v_full[st], (gl / kStages) & 1, ab, 6, kWaitCycles));
@@ -532,8 +574,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) tc::mbar_arrive(&v_clean[st]);
         }
         if (__any_sync(0xffffffffu, found) && lane == 0) {  // (both warps may note the unit: twice is as good as once)
-          const int i = atomicAdd(odd_count, 1);
-          if (i < kOddUnits) odd_units[i] = w.number;
+          if (w.piece >= 0) {
+            P.odd[w.number - P.whole] = 1;
+          } else {
+            const int i = atomicAdd(odd_count, 1);
+            if (i < kOddUnits) odd_units[i] = w.number;
+          }
         }
       }
     }
@@ -602,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int nb = t == 0 ? w.nblk0 : w.nblk1;
       float m_used = -INFINITY, l = 0.f;
       const uint32_t s_addr = tmem + lane_addr + tmem_s(t);
-      for (int j = 0; j < nb; ++j) {
+      for (int j = w.j0; j < nb; ++j) {
         if (!tc::mbar_wait(&s_full[t], sc & 1, ab, 4, kWaitCycles)) {
           ok = false;
           break;
@@ -706,7 +752,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += sum2.x + sum2.y;
       }
       if (!ok) break;
-      if (nb == 0) continue;  // no second tile
+      float *sums = P.partials + (int64_t)w.piece * kPieceFloats<D>;  // (of a piece)
+      const int prow = t * kBM + m;
+      if (w.piece >= 0) *reinterpret_cast<float2 *>(sums + kPieceRows * D + 2 * prow) = make_float2(m_used, l);
+      if (nb <= w.j0) continue;  // no second tile, or none of its blocks
       if (!tc::mbar_wait(&o_final[t], oc & 1, ab, 4, kWaitCycles)) break;
       ++oc;
       tc::fence_after_sync();
@@ -720,7 +769,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t x[32];
         tc::tmem_ld32(o_addr + c, x);
         tc::tmem_ld_wait();
-        if (valid) {
+        if (w.piece >= 0) {
+          if (valid)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<uint4 *>(sums + prow * D + c + 4 * i) =
+                  make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+        } else if (valid) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -742,10 +797,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   // second visit, or another CTA's unit, changes nothing: the values it adds are not finite.)
   const int n_odd = *odd_count;
   if (n_odd > 0) {
-    const int n = n_odd <= kOddUnits ? n_odd : (int)P.n_units;
+    const int n = n_odd <= kOddUnits ? n_odd : (int)P.whole;
     for (int i = 0; i < n; ++i) {
       Unit w;
-      if (!make_unit(P, n_odd <= kOddUnits ? odd_units[i] : i, w)) continue;
+      if (!make_item(P, n_odd <= kOddUnits ? odd_units[i] : i, w)) continue;
       for (int r = warp; r < 2 * kBM; r += kThreads / 32) {
         const int t = r / kBM, hh = r % kBM / P.Pt, pi = r % kBM % P.Pt;
         if (hh >= A.G || pi >= (t == 0 ? w.n0 : w.n1)) continue;
@@ -754,6 +809,60 @@ __global__ void __launch_bounds__(kThreads, 1)
                           reinterpret_cast<uint16_t *>(A.out.data) + (int64_t)tok * A.out.stride_token +
                               (int64_t)(w.g * A.G + hh) * A.out.stride_head);
       }
+    }
+  }
+}
+
+// Joins the pieces of the cut units: a warp takes a row, its lanes D / 32
+// elements each.  A piece's sums are relative to its own maximum; one in which
+// the row saw nothing (sum 0) was not written.
+constexpr int kJoinThreads = 256, kJoinRows = 16;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) join_pieces_kernel(const PrefillParams P) {
+  const AttendParams &A = P.a;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const unsigned cut = blockIdx.x;
+  Unit w;
+  if (!find_unit(P, (unsigned)P.whole + cut, w)) return;
+  const int nb = max(w.nblk0, w.nblk1), per = piece_blocks(P, nb), pieces = (nb + per - 1) / per;
+  for (int i = warp; i < kJoinRows; i += kJoinThreads / 32) {
+    const int r = blockIdx.y * kJoinRows + i, t = r / kBM, hh = r % kBM / P.Pt, pi = r % kBM % P.Pt;
+    if (hh >= A.G || pi >= (t == 0 ? w.n0 : w.n1)) continue;
+    const float *sums = P.partials + (int64_t)cut * P.splits * kPieceFloats<D>;
+    const float2 *stat = reinterpret_cast<const float2 *>(sums + kPieceRows * D) + r;
+    float top = -INFINITY;
+    for (int j = lane; j < pieces; j += 32) top = fmaxf(top, stat[j * (kPieceFloats<D> / 2)].x);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top > -INFINITY ? top : 0.f;
+    constexpr int kE = D / 32;
+    float l = 0.f, acc[kE];
+#pragma unroll
+    for (int e = 0; e < kE; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int j = 0; j < pieces; ++j) {
+      const float2 ml = stat[j * (kPieceFloats<D> / 2)];
+      if (ml.y == 0.f) continue;
+      const float f = ml.x > -INFINITY ? tc::ex2_approx(ml.x - base) : 1.f;  // (a NaN sum without a maximum stays)
+      l = fmaf(f, ml.y, l);
+      const float2 *x = reinterpret_cast<const float2 *>(sums + j * kPieceFloats<D> + r * D + lane * kE);
+#pragma unroll
+      for (int e = 0; e < kE; e += 2) {
+        const float2 v = x[e / 2];
+        acc[e] = fmaf(f, v.x, acc[e]), acc[e + 1] = fmaf(f, v.y, acc[e + 1]);
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int tok = w.tok + t * P.Pt + pi;
+    uint16_t *orow = reinterpret_cast<uint16_t *>(A.out.data) + (int64_t)tok * A.out.stride_token +
+                     (int64_t)(w.g * A.G + hh) * A.out.stride_head;
+#pragma unroll
+    for (int e = 0; e < kE; e += 2)
+      *reinterpret_cast<uint32_t *>(orow + lane * kE + e) = pack_any(acc[e] * inv, acc[e + 1] * inv, P.dtype);
+    if (P.odd[cut]) {
+      Unit all = w;
+      find_holes(A, all);
+      __syncwarp();
+      add_odd_values<D>(A, P.dtype, all, load_position(A.batch, tok), orow);
     }
   }
 }
@@ -856,11 +965,44 @@ int heads_at_once(const AttendParams &A) {
 }
 constexpr int64_t kMaxHeadBytes = 4ll << 30;
 
+// Which units are cut, and into how many pieces.  Lengths are not known here,
+// so requests count as equally long and as long as their tables.  In the time
+// of a block of 128 keys: a unit or piece takes its blocks and three more, and
+// a join about five.
+constexpr int kMaxPieces = 960;
+void cut_units(PrefillParams &P) {
+  const AttendParams &A = P.a;
+  const int64_t sms = sm_count(), batch = A.batch.batch, two = 2 * P.Pt;
+  const int64_t each = (A.batch.n_tokens + batch - 1) / batch;
+  const int64_t units = std::min(P.n_units, batch * ((each + two - 1) / two) * P.heads);
+  int64_t seen = held_keys(A);
+  if (A.window < 0x7fffffff) seen = std::min(seen, (int64_t)A.window + A.sinks + each + kBN);
+  const double blocks = (double)((seen + kBN - 1) / kBN);
+  P.whole = P.n_items = P.n_units, P.splits = 1;
+  double best = (double)((units + sms - 1) / sms) * (blocks + 3);
+  const int64_t rounds = units / sms;
+  for (int64_t r = std::max<int64_t>(0, rounds - 1); r <= rounds; ++r) {
+    const int64_t rest = units - r * sms;
+    if (rest <= 0) continue;
+    const int64_t cut = (rest * P.n_units + units - 1) / units;  // slots without tokens lie among the others
+    for (int s = 2; s <= 256 && cut * s <= kMaxPieces && blocks > kPieceBlocks * (s - 1); ++s) {
+      const double cost =
+          r * (blocks + 3) + (double)((rest * s + sms - 1) / sms) * (std::max<double>(std::ceil(blocks / s), kPieceBlocks) + 3) + 5;
+      if (cost < best) best = cost, P.whole = P.n_units - cut, P.splits = s, P.n_items = P.whole + cut * s;
+    }
+  }
+}
+
 int set_units(PrefillParams &P) {
   P.Pt = kBM / P.a.G;
   P.slots = P.a.batch.n_tokens / (2 * P.Pt) + P.a.batch.batch;
   P.n_units = (int64_t)P.slots * P.heads;
-  return P.n_units < (1ll << 31) - 4096 ? SB_OK : SB_ERR_TOO_LARGE;
+  cut_units(P);
+  return P.n_items < (1ll << 31) - 4096 ? SB_OK : SB_ERR_TOO_LARGE;
+}
+
+int64_t partial_bytes(const PrefillParams &P) {
+  return P.splits == 1 ? 0 : (P.n_items - P.whole) * 4 * kPieceRows * (P.a.cache.head_dim + 2);
 }
 
 template <typename T, int D, bool CONVERT>
@@ -871,15 +1013,20 @@ int run(PrefillParams &P, const CUtensorMap &tk, const CUtensorMap &tv, int32_t 
   if (ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kSmem) != SB_OK) return SB_ERR_CUDA;
   P.next = reinterpret_cast<unsigned *>(workspace);
   P.status = status ? status : reinterpret_cast<int *>(workspace) + 1;
+  P.odd = reinterpret_cast<unsigned *>(workspace) + 32;
+  static_assert(kPrefillWorkspace >= 128 + 4 * kMaxPieces, "flags of the cut units");
   const cudaError_t e = cudaMemsetAsync(workspace, 0, kPrefillWorkspace, st);
   if (e != cudaSuccess) {
     set_last_cuda_error(e);
     return SB_ERR_CUDA;
   }
-  const int grid = (int)std::min<int64_t>(sm_count(), P.n_units);
+  const int grid = (int)std::min<int64_t>(sm_count(), P.n_items);
   const int slot = prof_before(st);
   kernel<<<grid, kThreads, S::kSmem, st>>>(tk, tv, P);
   prof_after(slot, st);
+  const int s = launch_status();
+  if (s != SB_OK || P.splits == 1) return s;
+  join_pieces_kernel<D><<<dim3((unsigned)(P.n_units - P.whole), kPieceRows / kJoinRows), kJoinThreads, 0, st>>>(P);
   return launch_status();
 }
 
@@ -903,6 +1050,7 @@ int run_rows(PrefillParams &P, int32_t *status, void *workspace, cudaStream_t st
     return SB_ERR_CUDA;
   const int s = set_units(P);
   if (s != SB_OK) return s;
+  P.partials = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + kPrefillWorkspace);
   return bf ? run<__nv_bfloat16, D, false>(P, tk, tv, status, workspace, st)
             : run<__half, D, false>(P, tk, tv, status, workspace, st);
 }
@@ -921,6 +1069,7 @@ int run_codes(PrefillParams &P, int32_t *status, void *workspace, cudaStream_t s
     const int64_t elems = (int64_t)A.batch.batch * P.heads * held * D;
     E.rows[0] = reinterpret_cast<__half *>(reinterpret_cast<char *>(workspace) + kPrefillWorkspace);
     E.rows[1] = E.rows[0] + elems;
+    P.partials = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + kPrefillWorkspace + head_bytes(A) * step);
     expand_kernel<D><<<(unsigned)(A.batch.batch * (held / kExpandKeys)), kExpandThreads, 0, st>>>(E);
     int s = launch_status();
     if (s != SB_OK) return s;
@@ -959,7 +1108,14 @@ bool prefill_takes(const AttendParams &P, int dtype) {
 }
 
 int64_t prefill_workspace_bytes(const AttendParams &P) {
-  return kPrefillWorkspace + (P.cache.group == 0 ? 0 : head_bytes(P) * heads_at_once(P));
+  // heads in groups: all of them but the last of one size
+  PrefillParams Q;
+  Q.a = P, Q.Pt = kBM / P.G;
+  const int step = P.cache.group == 0 ? P.cache.n_heads : heads_at_once(P);
+  int64_t partials = 0;
+  for (int heads : {step, P.cache.n_heads % step})
+    if (Q.heads = heads; heads > 0 && set_units(Q) == SB_OK) partials = std::max(partials, partial_bytes(Q));
+  return kPrefillWorkspace + (P.cache.group == 0 ? 0 : head_bytes(P) * step) + partials;
 }
 
 int launch_prefill(const AttendParams &A, int dtype, int32_t *status, void *workspace, cudaStream_t st) {
