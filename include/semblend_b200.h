@@ -508,12 +508,13 @@ SB_API int sb_paged_append(const sb_paged_cache *cache, const sb_paged_batch *ba
 SB_API int sb_paged_gather(const sb_paged_cache *cache, const sb_paged_batch *batch, sb_token_rows key_out,
                            sb_token_rows value_out, int32_t dtype, uint64_t *err_counter, void *stream);
 
-/* Device bytes sb_paged_attention needs (128-byte aligned); -1 for invalid
- * arguments.  One workspace serves one call at a time.  Many query rows over
+/* Device bytes sb_paged_attention needs (128-byte aligned) with these sizes,
+ * strides and mask; -1 for invalid arguments.  One workspace serves one call at a time.  Many query rows over
  * a 4-bit cache are served from fp16 copies of the keys they see: up to 1 GiB
  * of them, or one KV head's where that is more. */
 SB_API int64_t sb_paged_attention_workspace_bytes(const sb_paged_cache *cache, const sb_paged_batch *batch,
-                                                  int32_t n_q_heads, int32_t dtype);
+                                                  int32_t n_q_heads, int32_t window, int32_t sinks,
+                                                  int32_t dtype);
 
 /* Attention of each token's query rows over its request's cached rows: key j
  * is visible at position p when j <= p, j addresses a row and, with window >

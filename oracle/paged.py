@@ -139,11 +139,10 @@ def attention(query, cache, tables, cu, positions, window=None, sinks=0, scale=N
             continue
         page = tables[b, j // bs].long()
         kv = cache[page, :, :, j % bs].double()  # [J, 2, H, D]
-        for h in range(Hq):
-            q, k, v = query[t, h].double(), kv[:, 0, h // (Hq // H)], kv[:, 1, h // (Hq // H)]
-            s = (k @ q) * scale
-            w = torch.exp(s - s.max())
-            w = w / w.sum()
-            out[t, h], spread[t, h] = w @ v, w @ v.abs()
-            reach[t, h] = (k.abs() @ q.abs()).max() * abs(scale)
+        q, k, v = query[t].double().unflatten(0, (H, -1)), kv[:, 0].transpose(0, 1), kv[:, 1].transpose(0, 1)
+        x = (q @ k.mT) * scale  # [H, Hq / H, J]
+        w = torch.exp(x - x.amax(-1, keepdim=True))
+        w = w / w.sum(-1, keepdim=True)
+        out[t], spread[t] = (w @ v).flatten(0, 1), (w @ v.abs()).flatten(0, 1)
+        reach[t] = (q.abs() @ k.abs().mT).amax(-1).flatten() * abs(scale)
     return out, spread, reach

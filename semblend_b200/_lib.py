@@ -247,7 +247,9 @@ _SIGNATURES: dict[str, tuple] = {
          ctypes.c_void_p],
     ),
     "sb_paged_attention_workspace_bytes": (
-        ctypes.c_int64, [_P(SbPagedCache), _P(SbPagedBatch), ctypes.c_int32, ctypes.c_int32]),
+        ctypes.c_int64,
+        [_P(SbPagedCache), _P(SbPagedBatch), ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32],
+    ),
     "sb_paged_attention": (
         ctypes.c_int,
         [_P(SbPagedCache), _P(SbPagedBatch), SbTokenRows, SbTokenRows, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,

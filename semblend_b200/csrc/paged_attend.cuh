@@ -142,13 +142,14 @@ template <int D> __device__ __forceinline__ void clear(RowSums<D> &r) {
   for (int i = 0; i < D / 32; ++i) r.acc[i] = 0.f;
 }
 // Decode path (csrc/paged_decode.cu): tiles of 8 or 16 query rows, keys split over CTAs.
+int64_t decode_tiles(const AttendParams &P);  // of 8 or 16 rows, requests taken as equally long
 bool decode_takes(const AttendParams &P, int dtype);
 int64_t decode_workspace_bytes(const AttendParams &P);
 int launch_decode(const AttendParams &P, int dtype, void *workspace, cudaStream_t st);
 
 
 // Prefill path (csrc/paged_prefill.cu): tiles of 128 query rows on tcgen05.
-constexpr int kPrefillWorkspace = 4096;  // unit counter and status, ahead of expanded rows
+constexpr int kPrefillWorkspace = 4096;  // unit counter, status and flags, ahead of rows and sums
 int64_t prefill_workspace_bytes(const AttendParams &P);
 bool prefill_takes(const AttendParams &P, int dtype);
 int launch_prefill(const AttendParams &P, int dtype, int32_t *status, void *workspace, cudaStream_t st);

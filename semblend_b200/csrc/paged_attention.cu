@@ -112,16 +112,19 @@ int launch_simt(const AttendParams &P, cudaStream_t st) {
 }  // namespace sb
 
 extern "C" SB_API int64_t sb_paged_attention_workspace_bytes(const sb_paged_cache *cache, const sb_paged_batch *batch,
-                                                             int32_t n_q_heads, int32_t dtype) {
+                                                             int32_t n_q_heads, int32_t window, int32_t sinks,
+                                                             int32_t dtype) {
   using namespace sb;
   if (paged::check_cache(cache) != SB_OK || paged::check_batch(batch) != SB_OK || n_q_heads <= 0 ||
-      n_q_heads % cache->n_heads || !elem_bytes(dtype))
+      n_q_heads % cache->n_heads || window < 0 || sinks < 0 || !elem_bytes(dtype))
     return -1;
   if (batch->batch == 0 || batch->n_tokens == 0) return 0;
   paged::AttendParams P = {};
   P.cache = *cache, P.batch = *batch;
   P.Hq = n_q_heads, P.G = n_q_heads / cache->n_heads;
-  P.scale = 1.f, P.window = 0x7fffffff;  // a window only makes the call need less
+  P.scale = 1.f;
+  P.window = window ? window : 0x7fffffff, P.sinks = window ? sinks : 0;
+  // rows count as aligned here: one path's need is no less than none
   if (paged::prefill_takes(P, dtype))  // with a scale of 0 the decode path takes the call
     return std::max(paged::decode_workspace_bytes(P), paged::prefill_workspace_bytes(P));
   return paged::decode_takes(P, dtype) ? paged::decode_workspace_bytes(P) : 0;

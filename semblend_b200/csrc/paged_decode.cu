@@ -1010,6 +1010,12 @@ int64_t cut_bytes(const AttendParams &A) {
 }
 }  // namespace
 
+int64_t decode_tiles(const AttendParams &A) {
+  const DecodeParams P = plan(A, SB_DTYPE_BF16);
+  const int64_t each = ((int64_t)A.batch.n_tokens + A.batch.batch - 1) / A.batch.batch;
+  return A.batch.batch * ((each + P.tokens_per_tile - 1) / P.tokens_per_tile) * P.head_tiles * A.cache.n_heads;
+}
+
 int64_t decode_workspace_bytes(const AttendParams &P) {
   if (plan(P, SB_DTYPE_BF16).whole) return 0;
   return cut_bytes(P) + (int64_t)max_grid(P, kMaxResident) * 2 * 16 * (P.cache.head_dim + 2) * 4;

@@ -71,6 +71,7 @@ struct PrefillParams {
   // item is a unit below `whole`, then a piece
   int64_t whole, n_items;
   int splits;
+  double cost;           // estimated (host)
   float *partials;       // workspace: of each piece 256 rows of D sums, then 256 pairs of maximum and sum
   int pages, page_rows;  // pages of a block of 128 keys and the rows a box takes of one
   int linear;            // 1: rows expanded to the workspace, [request][head - head0][key]
@@ -965,22 +966,33 @@ int heads_at_once(const AttendParams &A) {
 }
 constexpr int64_t kMaxHeadBytes = 4ll << 30;
 
-// Which units are cut, and into how many pieces.  Lengths are not known here,
-// so requests count as equally long and as long as their tables.  In the time
-// of a block of 128 keys: a unit or piece takes its blocks and three more, and
-// a join about five.
+// Blocks of 128 keys that a tile goes through, at most.  Lengths are not known on the host: requests count
+// as equally long, and as long as their tables.
+int64_t tokens_each(const AttendParams &A) { return ((int64_t)A.batch.n_tokens + A.batch.batch - 1) / A.batch.batch; }
+int64_t seen_blocks(const AttendParams &A) {
+  int64_t seen = held_keys(A);
+  if (A.window < 0x7fffffff) seen = std::min(seen, (int64_t)A.window + A.sinks + tokens_each(A) + kBN);
+  return (seen + kBN - 1) / kBN;
+}
+
+// Which units are cut, and into how many pieces; returns the time estimated, in
+// that of a block (2 us): a unit or piece takes its blocks and three more, and
+// a join about five.  (28/4 heads: 64 tokens at the end of 32K 544 us with
+// whole units, 75 cut; 4,096 tokens, 3.08 rounds of units, 1,989 and 1,592.)
+// Tokens that are the greater part of their context see ever less towards the
+// first ones, which come last and even the ends out by themselves: 8,192 of 8K
+// (8/8 heads) took 166 us whole, 191 cut.
 constexpr int kMaxPieces = 960;
-void cut_units(PrefillParams &P) {
+double cut_units(PrefillParams &P) {
   const AttendParams &A = P.a;
   const int64_t sms = sm_count(), batch = A.batch.batch, two = 2 * P.Pt;
-  const int64_t each = (A.batch.n_tokens + batch - 1) / batch;
+  const int64_t each = tokens_each(A);
   const int64_t units = std::min(P.n_units, batch * ((each + two - 1) / two) * P.heads);
-  int64_t seen = held_keys(A);
-  if (A.window < 0x7fffffff) seen = std::min(seen, (int64_t)A.window + A.sinks + each + kBN);
-  const double blocks = (double)((seen + kBN - 1) / kBN);
+  const double blocks = (double)seen_blocks(A);
   P.whole = P.n_items = P.n_units, P.splits = 1;
   double best = (double)((units + sms - 1) / sms) * (blocks + 3);
   const int64_t rounds = units / sms;
+  if (A.window == 0x7fffffff && 2 * each > held_keys(A)) return best;
   for (int64_t r = std::max<int64_t>(0, rounds - 1); r <= rounds; ++r) {
     const int64_t rest = units - r * sms;
     if (rest <= 0) continue;
@@ -991,13 +1003,14 @@ void cut_units(PrefillParams &P) {
       if (cost < best) best = cost, P.whole = P.n_units - cut, P.splits = s, P.n_items = P.whole + cut * s;
     }
   }
+  return best;
 }
 
 int set_units(PrefillParams &P) {
   P.Pt = kBM / P.a.G;
   P.slots = P.a.batch.n_tokens / (2 * P.Pt) + P.a.batch.batch;
   P.n_units = (int64_t)P.slots * P.heads;
-  cut_units(P);
+  P.cost = cut_units(P);
   return P.n_items < (1ll << 31) - 4096 ? SB_OK : SB_ERR_TOO_LARGE;
 }
 
@@ -1089,8 +1102,8 @@ int run_codes(PrefillParams &P, int32_t *status, void *workspace, cudaStream_t s
 
 }  // namespace
 
-// Enough rows per request to fill tiles of 128; pages that cut a block of 128 keys evenly, in whole swizzle
-// groups of 8 rows.
+// Pages that cut a block of 128 keys evenly, in whole swizzle groups of 8 rows, and enough rows that this path
+// takes less time than the other's tiles of 16 rows.
 bool prefill_takes(const AttendParams &P, int dtype) {
   if (!decode_takes(P, dtype) || P.G > kBM || P.scale == 0.f || P.batch.max_blocks == 0) return false;
   if (!rows_aligned(P.out, 2, 16)) return false;
@@ -1104,13 +1117,27 @@ bool prefill_takes(const AttendParams &P, int dtype) {
   if (P.cache.group != 0 && (held_keys(P) >= (1ll << 31) || head_bytes(P) > kMaxHeadBytes ||
                              P.batch.batch * (held_keys(P) / kExpandKeys) >= (1ll << 31)))
     return false;
-  return (int64_t)P.batch.n_tokens * P.G >= 64 * (int64_t)P.batch.batch;
+  // one tile of 16 rows per request is always faster there (2 tokens, 28/4 heads, 32K: 36 and 48 us, 8 requests
+  // 106 and 154)
+  if ((int64_t)P.batch.n_tokens * P.G <= 16 * (int64_t)P.batch.batch) return false;
+  // Estimates in us (codes: the expansion is the third term), fitted to 1 to 64 requests of 1K to 32K keys.  16-bit
+  // rows, the other path and this one: 1 x 32K
+  // keys, 4 tokens 43 and 48, 8 tokens 60 and 50, 64 tokens 333 and 75; 1 x 1K, 64 tokens 33 and 35; 8 x 8K, 4
+  // tokens 61 and 62, 16 tokens 179 and 68; 64 x 1K, 2 tokens 37 and 54, 4 tokens 64 and 54.  Codes: 1 x 32K, 16
+  // tokens 84 and 107, 32 tokens 148 and 113; 8 x 32K, 10 tokens 332 and 377, 16 tokens 516 and 381.
+  const double blocks = (double)seen_blocks(P);
+  PrefillParams Q;
+  Q.a = P, Q.heads = P.cache.n_heads;
+  if (set_units(Q) != SB_OK) return true;
+  const double here = 13 + 2 * Q.cost + (c.group == 0 ? 0 : 20 + 0.0214 * c.n_heads * (double)P.batch.batch * blocks);
+  const double there = 22 + (c.group == 0 ? 1.4 : 1.15) * (double)decode_tiles(P) * blocks / sm_count();
+  return here < there;
 }
 
 int64_t prefill_workspace_bytes(const AttendParams &P) {
   // heads in groups: all of them but the last of one size
   PrefillParams Q;
-  Q.a = P, Q.Pt = kBM / P.G;
+  Q.a = P;
   const int step = P.cache.group == 0 ? P.cache.n_heads : heads_at_once(P);
   int64_t partials = 0;
   for (int heads : {step, P.cache.n_heads % step})

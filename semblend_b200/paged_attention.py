@@ -398,7 +398,7 @@ def paged_attention(
         if status.dtype != torch.int32 or status.numel() < 1:
             raise TypeError("status must be an int32 tensor of one element")
     lib = _lib.load()
-    nbytes = lib.sb_paged_attention_workspace_bytes(c, batch._c, hq, code)
+    nbytes = lib.sb_paged_attention_workspace_bytes(c, batch._c, hq, window or 0, sinks, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
     _call(dev, "paged_attention", lib.sb_paged_attention, c, batch._c, q, o, hq, window or 0, sinks, scale, code,
           None if ws is None else ws.data_ptr(), nbytes, None if status is None else status.data_ptr())

@@ -154,11 +154,11 @@ def test_entry_points_refuse_bad_geometry(group):
 def test_workspace_size_refuses_what_the_call_refuses():
     lib = _lib.load()
     c, b = _structs()
-    assert lib.sb_paged_attention_workspace_bytes(c, b, 4, _lib.SB_DTYPE_BF16) >= 0
-    assert lib.sb_paged_attention_workspace_bytes(c, b, 3, _lib.SB_DTYPE_BF16) == -1
-    assert lib.sb_paged_attention_workspace_bytes(c, b, 4, 5) == -1
+    assert lib.sb_paged_attention_workspace_bytes(c, b, 4, 0, 0, _lib.SB_DTYPE_BF16) >= 0
+    assert lib.sb_paged_attention_workspace_bytes(c, b, 3, 0, 0, _lib.SB_DTYPE_BF16) == -1
+    assert lib.sb_paged_attention_workspace_bytes(c, b, 4, 0, 0, 5) == -1
     c.block_size = 0
-    assert lib.sb_paged_attention_workspace_bytes(c, b, 4, _lib.SB_DTYPE_BF16) == -1
+    assert lib.sb_paged_attention_workspace_bytes(c, b, 4, 0, 0, _lib.SB_DTYPE_BF16) == -1
     assert lib.sb_paged_append(None, b, *[_lib.SbTokenRows()] * 4, 0, 2, None, 0, None, None) == INV
     assert lib.sb_paged_append(c, None, *[_lib.SbTokenRows()] * 4, 0, 2, None, 0, None, None) == INV
 

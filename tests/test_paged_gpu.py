@@ -498,6 +498,69 @@ def test_long_context(group, new):
     attend(c) if new < 10 else attend(c, window=1000, sinks=64)
 
 
+TILED = [(28, 4, 128, 16, "canonical"), (64, 8, 64, 32, "vllm"), (16, 16, 128, 128, "trtllm"),
+         (32, 4, 128, 256, "canonical"), (40, 1, 64, 8, "canonical")]
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (33, 4), (300, 130)])
+@pytest.mark.parametrize("dtype,group", [(BF, None), (HF, None), (BF, 64), (HF, 32), (BF, "D")])
+@pytest.mark.parametrize("hq,h,d,bs,layout", TILED)
+def test_attention_many_rows(hq, h, d, bs, layout, dtype, group, window, sinks):
+    """Enough rows for tiles of 128; pages below, at and above a block of 128 keys."""
+    c = Case(ctx=[700, 513, 640, 1], new=[150, 97, 160, 0], dtype=dtype, hq=hq, h=h, d=d, bs=bs,
+             group=d if group == "D" else group, seed=23, pad=2)
+    attend(c, layout, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (700, 4), (1500, 300)])
+@pytest.mark.parametrize("dtype,group", [(BF, None), (HF, None), (BF, 64), (HF, 32)])
+@pytest.mark.parametrize("hq,h,d,spread", [(28, 4, 128, False), (28, 4, 128, True), (16, 16, 64, False)])
+def test_attention_cut_along_the_keys(hq, h, d, spread, dtype, group, window, sinks):
+    """Few tiles over long contexts: each is cut into pieces, some without a key for a row."""
+    c = Case(ctx=[2600, 1900, 1281], new=[150, 97, 130], dtype=dtype, hq=hq, h=h, d=d, group=group, seed=24,
+             spread=spread)
+    attend(c, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("group", [None, 64])
+def test_cut_along_the_keys_with_holes(group):
+    """Unmapped pages, a whole piece without any page, tokens that see nothing, positions in any order."""
+    c = Case(ctx=[2600, 1900], new=[150, 97], hq=28, h=4, group=group, seed=25, spread=True, table=torch.int64)
+    c.tables[0, 3] = -1
+    c.tables[0, 40] = c.nb + 9
+    c.tables[0, 64:130] = -1
+    c.tables[1, :70] = -1
+    c.positions[3] = -1
+    c.positions[:150] = c.positions[torch.randperm(150)]
+    attend(c)
+    attend(c, window=900, sinks=70)
+    c.tables[1, :] = -1
+    attend(c)
+
+
+@pytest.mark.parametrize("new", [200, 400])
+def test_cut_along_the_keys_keeps_odd_values_apart(new):
+    """Infinities and NaN of V and K reach exactly the tokens that see them."""
+    c = Case(ctx=[2600], new=[new], hq=28, h=4, seed=26)
+    clean = c.cache.clone()
+    for j, what, kv in ((2450, float("inf"), 0), (2520, float("nan"), 0), (2580, float("nan"), 1)):
+        at = int(c.tables[0, j // 16]), 1 - kv, 2, j % 16, 3
+        c.cache[at], clean[at] = what, 0.0
+    out = paged_attention(c.q.to(DEV), c.device_cache(), c.batch()).cpu().double()
+    c.cache = clean
+    want, spread, _ = op.attention(c.q, clean, c.tables, c.cu, c.positions)
+    pos = c.positions
+    heads = slice(14, 21)  # of KV head 2
+    assert torch.all(out[(pos >= 2450) & (pos < 2520), heads, 3] == float("inf"))
+    assert torch.all(out[(pos >= 2520) & (pos < 2580), heads, 3].isnan())
+    assert torch.all(out[pos >= 2580, heads].isnan())
+    ok = torch.ones_like(out, dtype=torch.bool)
+    ok[pos >= 2450, heads, 3] = False
+    ok[pos >= 2580, heads] = False
+    tol = U[BF] * want.abs() + (U[BF] + 2.0**-12) * spread
+    assert torch.all(((out - want).abs() <= tol)[ok])
+
+
 def test_rows_past_32_bits():
     """A pool whose rows lie more than 2^31 elements from its start."""
     h, d, bs = 1, 128, 16
