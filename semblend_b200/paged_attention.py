@@ -366,8 +366,9 @@ def paged_attention(
     ``j > p - window`` or ``j < sinks``.  The new tokens' own rows must be in
     the cache first (:func:`append_paged_kv`).  Softmax statistics and sums are
     fp32.  A token that sees no key gives zeros; what unseen rows hold (NaN
-    and infinities included) has no effect.  Padding rows stay as they were in
-    ``out``, and zero in a new result.  ``status`` (device int32) receives a
+    and infinities included) has no effect.  Without a window ``sinks`` change
+    nothing.  Padding rows stay as they were in ``out``, which may be
+    ``query`` itself, and zero in a new result.  ``status`` (device int32) receives a
     value >= 2 if a kernel wait timed out.
     """
     c = _cache(kv_cache, batch, layout)

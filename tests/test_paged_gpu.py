@@ -561,6 +561,78 @@ def test_cut_along_the_keys_keeps_odd_values_apart(new):
     assert torch.all(((out - want).abs() <= tol)[ok])
 
 
+@pytest.mark.parametrize("group", [None, 64])
+@pytest.mark.parametrize("new,d", [(1, 128), (3, 128), (180, 128), (40, 80)])
+def test_out_may_be_the_query(new, d, group):
+    """One token, a few, tiles cut along the keys, and the path of other head dims."""
+    if d == 80 and group:
+        pytest.skip("4-bit rows have 64 or 128 elements")
+    c = Case(ctx=[1700, 1300], new=[new, new], hq=28, h=4, d=d, group=group, seed=27)
+    q = c.q.to(DEV)
+    assert paged_attention(q, c.device_cache(), c.batch(), window=1500, sinks=4, out=q) is q
+    check_attention(c, q, window=1500, sinks=4)
+
+
+def test_many_tiles_with_odd_values():
+    """More tiles with a NaN in V than a CTA keeps a list of."""
+    B, n, h, hq, d = 2600, 20, 8, 64, 64
+    g = torch.Generator(device=DEV).manual_seed(28)
+    cache = torch.randn(B, 2, h, 32, d, generator=g, device=DEV).to(BF)
+    cache[:, 1, :, 5, 3] = float("nan")
+    cache[:, :, :, n:] = float("inf")  # behind the last token
+    q = torch.randn(B * n, hq, d, generator=g, device=DEV).to(BF)
+    batch = PagedBatch(torch.randperm(B, generator=g, device=DEV).int()[:, None],
+                       torch.arange(B + 1, dtype=torch.int32, device=DEV) * n,
+                       torch.arange(n, dtype=torch.int32, device=DEV).repeat(B))
+    out = paged_attention(q, cache, batch).view(B, n, hq, d)
+    assert torch.all(out[:, :5].isfinite()) and torch.all(out[:, 5:, :, 3].isnan())
+    out[..., 3] = 0
+    assert torch.all(out.isfinite())
+    assert torch.equal(out[:, 0, :, 4:], cache[batch.block_tables[:, 0].long(), 1, :, 0, 4:].repeat_interleave(8, 1))
+
+
+@pytest.mark.parametrize("group", [None, 32])
+@pytest.mark.parametrize("offset", [0, 1, 4])
+def test_gather_into_rows_of_any_stride(group, offset):
+    c = Case(ctx=[60, 33], new=[23, 33], hq=2, h=2, d=64, group=group, seed=29)
+    wide = torch.full((2, c.h, c.T, 70), 5.0, dtype=BF, device=DEV)
+    out = wide[..., offset : offset + 64]
+    gather_paged_kv(c.device_cache(), c.batch(), out=out)
+    src = c.value_cache()
+    for t, (_, page, row) in enumerate(op.rows_of(c.tables, c.cu, c.positions, c.bs, c.nb)):
+        assert torch.equal(out[:, :, t].cpu(), src[page, :, :, row].float().to(BF))
+    rest = torch.cat([wide[..., :offset], wide[..., offset + 64 :]], -1)
+    assert torch.all(rest == 5.0)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_append4_unaligned_rows_and_query_in_place(dtype):
+    c = Case(ctx=[70, 20], new=[33, 20], dtype=dtype, hq=3, h=1, d=64, group=32, seed=30)
+    fused = torch.randn(c.T, 5, 67, generator=torch.Generator().manual_seed(31)).to(dtype)
+    dev = fused.to(DEV)
+    cache = c.device_cache()
+    append_paged_kv(cache, dev[:, 3:4, 3:], dev[:, 4:, 1:65], c.batch(), 1e5, query=dev[:, :3, 2:66],
+                    query_out=dev[:, :3, 2:66], rotary_style="neox")
+    assert op.append4(c.codes, c.scales, fused[:, 3:4, 3:], fused[:, 4:, 1:65], c.tables, c.cu, c.positions, 1e5,
+                      "neox") == 0
+    assert torch.equal(op.unpack(cache.codes.cpu()), c.codes) and torch.equal(cache.scales.cpu(), c.scales)
+    exact = op.rotate(fused[:, :3, 2:66], c.positions, 1e5, "neox")
+    diff = (dev[:, :3, 2:66].cpu().double() - exact).abs()
+    assert torch.all(diff <= rope_tolerance(fused[:, :3, 2:66], exact, "neox", U[dtype]))
+    dev[:, :3, 2:66] = fused[:, :3, 2:66].to(DEV)
+    assert torch.equal(dev.cpu(), fused)
+
+
+@pytest.mark.parametrize("group", [None, 64])
+@pytest.mark.parametrize("new", [1, 2, 180])
+def test_wide_table_and_short_window(new, group):
+    """A table far wider than the contexts, a window of a few tiles: what is cut follows the window."""
+    c = Case(ctx=[1500, 900], new=[new, new], hq=28, h=4, group=group, seed=32)
+    c.tables = torch.cat([c.tables, torch.full((2, 2500), -1, dtype=c.tables.dtype)], 1)
+    for window, sinks in ((None, 0), (200, 4), (1100, 200)):
+        attend(c, window=window, sinks=sinks)
+
+
 def test_rows_past_32_bits():
     """A pool whose rows lie more than 2^31 elements from its start."""
     h, d, bs = 1, 128, 16
