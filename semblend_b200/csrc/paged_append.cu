@@ -5,10 +5,18 @@
 //     K'(2 elements of RoPE pair i) = (x1 cos - x2 sin, x2 cos + x1 sin),
 //     angle = p * inv_freq[i],
 // and its V row to row (table[b][p / bs], p % bs); query rows are rotated
-// beside it.  All three kernels move each byte once and are bound by HBM (by
-// launch latency for a decode step): a CTA takes a few tokens, computes their
-// angles once for all heads into shared memory, and its threads move two
-// vectors of up to 16 bytes per row, the two halves the neox pairs lie in.
+// beside it.  The kernels move each byte once and are bound by HBM (by launch
+// latency for a decode step): a CTA takes a few tokens, computes their angles
+// once for all heads into shared memory, and its threads move two vectors of up
+// to 16 bytes per row, the two halves the neox pairs lie in.
+//
+// Measured (replayed graphs): 16,384 tokens of 28/4 heads of 128 in bf16, query
+// rotated beside, 52 us, 5.8 TB/s of a copy's 6.45 (8 CTAs an SM with 32
+// registers a thread; with 48 registers 57); a decode step 4 us.  4-bit rows of
+// such a chunk take 43 us where its bytes would take 13: the rotation in 64
+// bits, which makes the codes a function of the input alone, and the packing
+// bound it (58 before divisions by runtime sizes and the slow conversions were
+// taken out).
 #include <algorithm>
 
 #include "paged.cuh"

@@ -16,10 +16,21 @@
 //                 the unit sees are loaded from behind the pool, as zeros
 //   4-bit codes   expand_kernel first writes the keys that the call sees to the
 //                 workspace as fp16 rows, some KV heads at a time, and the same
-//                 kernel runs on those in fp16.  A key is then expanded once,
+//                 kernel runs on those in fp16: a key is off by half an fp16
+//                 step, as it would be in an fp16 cache.  A key is then expanded once,
 //                 not once per unit: with the expansion in the loading warps
 //                 the kernel was bound by instruction issue, 980 us for 2,048
 //                 tokens over 16K (28/4 heads)
+//
+// Units that do not fill the GPU evenly are cut along the keys, into pieces
+// that leave fp32 sums with their maximum and sum, joined by a second kernel.
+//
+// Measured (replayed graphs): 3,277 scattered tokens over 32K keys, window 4,096,
+// 28/4 heads, 308 us, 0.36 of the matrix rate by visible pairs (a unit goes
+// through all blocks that one of its tokens sees); 4,096 tokens at the end of
+// 32K 1,592 us, 0.66; from 4-bit rows 2,048 tokens of 16K 531 us, 0.50, of them
+// about 50 the expansion.  The chain softmax, P.V, next S of a tile bounds a
+// block, 2 us for two tiles, as in the dense kernel.
 //
 // A key that a row does not see has its score replaced.  Its V row must not
 // reach the products as an infinity or a NaN (zero times it is a NaN): in the
@@ -1120,11 +1131,11 @@ bool prefill_takes(const AttendParams &P, int dtype) {
   // one tile of 16 rows per request is always faster there (2 tokens, 28/4 heads, 32K: 36 and 48 us, 8 requests
   // 106 and 154)
   if ((int64_t)P.batch.n_tokens * P.G <= 16 * (int64_t)P.batch.batch) return false;
-  // Estimates in us (codes: the expansion is the third term), fitted to 1 to 64 requests of 1K to 32K keys.  16-bit
-  // rows, the other path and this one: 1 x 32K
-  // keys, 4 tokens 43 and 48, 8 tokens 60 and 50, 64 tokens 333 and 75; 1 x 1K, 64 tokens 33 and 35; 8 x 8K, 4
-  // tokens 61 and 62, 16 tokens 179 and 68; 64 x 1K, 2 tokens 37 and 54, 4 tokens 64 and 54.  Codes: 1 x 32K, 16
-  // tokens 84 and 107, 32 tokens 148 and 113; 8 x 32K, 10 tokens 332 and 377, 16 tokens 516 and 381.
+  // Estimates in us (codes: the expansion is the third term), fitted to 1 to 64 requests of 1K to 32K keys.
+  // 16-bit rows, the other path and this one: 1 x 32K keys, 4 tokens 43 and 48, 8 tokens 60 and 50, 64 tokens
+  // 333 and 75; 1 x 1K, 64 tokens 33 and 35; 8 x 8K, 4 tokens 61 and 62, 16 tokens 179 and 68; 64 x 1K, 2 tokens
+  // 37 and 54, 4 tokens 64 and 54.  Codes: 1 x 32K, 16 tokens 84 and 107, 32 tokens 148 and 113; 8 x 32K, 10
+  // tokens 332 and 377, 16 tokens 516 and 381.
   const double blocks = (double)seen_blocks(P);
   PrefillParams Q;
   Q.a = P, Q.heads = P.cache.n_heads;
