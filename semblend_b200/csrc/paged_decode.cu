@@ -24,14 +24,14 @@
 // Short contexts are not cut: a cluster of up to eight CTAs takes a tile whole
 // and joins it over distributed shared memory, in the same launch.
 //
-// Measured (replayed graphs; HBM copies at 6.45 TB/s): 64 requests of 2K to 32K
-// keys, 64/8 heads, 16-bit rows 179 us, 6.0 TB/s; one request of 32K and 8 new
-// tokens a step 96 us, 5.5 TB/s; one request of 517 keys 9.4 us, latency.  Over
+// Measured (one new token each, replayed graphs; HBM copies at 6.45 TB/s): 64
+// requests of 4K to 32K keys, window 4,096, 64/8 heads, 177 us, 6.1 TB/s; eight
+// of 20K to 32K, 28/4 heads, 96 us, 5.5 TB/s; one of 517 9.4 us, latency.  Over
 // 4-bit rows the loads are no longer the bound but instruction issue and its
 // latency at 12 warps an SM: about 700 instructions for 32 keys of a warp, which
 // become fp16 subnormals (a shift and a mask for two codes), so that the step
 // and the zero of a group apply to the products and not to each element; the
-// same 64 requests take 307 us, 3.5 TB/s of codes.  (16 keys at a time: 362; four
+// 64 requests without the window take 307 us, 3.5 TB/s.  (16 keys at a time: 362; four
 // CTAs an SM with two stages: 294 to 306.)
 #include <algorithm>
 #include <type_traits>

@@ -26,9 +26,9 @@
 // that leave fp32 sums with their maximum and sum, joined by a second kernel.
 //
 // Measured (replayed graphs): 3,277 scattered tokens over 32K keys, window 4,096,
-// 28/4 heads, 308 us, 0.36 of the matrix rate by visible pairs (a unit goes
+// 28/4 heads, 299 us, 0.37 of the matrix rate by visible pairs (a unit goes
 // through all blocks that one of its tokens sees); 4,096 tokens at the end of
-// 32K 1,592 us, 0.66; from 4-bit rows 2,048 tokens of 16K 531 us, 0.50, of them
+// 32K 1,593 us, 0.66; from 4-bit rows 2,048 tokens of 16K 515 us, 0.51, of them
 // about 50 the expansion.  The chain softmax, P.V, next S of a tile bounds a
 // block, 2 us for two tiles, as in the dense kernel.
 //
@@ -826,9 +826,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the pieces of the cut units: a warp takes a row, its lanes D / 32
-// elements each.  A piece's sums are relative to its own maximum; one in which
-// the row saw nothing (sum 0) was not written.
-constexpr int kJoinThreads = 256, kJoinRows = 16;
+// elements each.  A piece's sums are relative to its own maximum; those of one
+// in which the row saw nothing (sum 0) were not written and are not used.
+constexpr int kJoinThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) join_pieces_kernel(const PrefillParams P) {
   const AttendParams &A = P.a;
@@ -837,8 +837,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_pieces_kernel(const Prefill
   Unit w;
   if (!find_unit(P, (unsigned)P.whole + cut, w)) return;
   const int nb = max(w.nblk0, w.nblk1), per = piece_blocks(P, nb), pieces = (nb + per - 1) / per;
-  for (int i = warp; i < kJoinRows; i += kJoinThreads / 32) {
-    const int r = blockIdx.y * kJoinRows + i, t = r / kBM, hh = r % kBM / P.Pt, pi = r % kBM % P.Pt;
+  const int rows = kPieceRows / gridDim.y;
+  for (int i = warp; i < rows; i += kJoinThreads / 32) {
+    const int r = blockIdx.y * rows + i, t = r / kBM, hh = r % kBM / P.Pt, pi = r % kBM % P.Pt;
     if (hh >= A.G || pi >= (t == 0 ? w.n0 : w.n1)) continue;
     const float *sums = P.partials + (int64_t)cut * P.splits * kPieceFloats<D>;
     const float2 *stat = reinterpret_cast<const float2 *>(sums + kPieceRows * D) + r;
@@ -853,14 +854,14 @@ __global__ void __launch_bounds__(kJoinThreads) join_pieces_kernel(const Prefill
 #pragma unroll 4
     for (int j = 0; j < pieces; ++j) {
       const float2 ml = stat[j * (kPieceFloats<D> / 2)];
-      if (ml.y == 0.f) continue;
+      const bool some = ml.y != 0.f;
       const float f = ml.x > -INFINITY ? tc::ex2_approx(ml.x - base) : 1.f;  // (a NaN sum without a maximum stays)
-      l = fmaf(f, ml.y, l);
+      if (some) l = fmaf(f, ml.y, l);
       const float2 *x = reinterpret_cast<const float2 *>(sums + j * kPieceFloats<D> + r * D + lane * kE);
 #pragma unroll
       for (int e = 0; e < kE; e += 2) {
         const float2 v = x[e / 2];
-        acc[e] = fmaf(f, v.x, acc[e]), acc[e + 1] = fmaf(f, v.y, acc[e + 1]);
+        acc[e] = some ? fmaf(f, v.x, acc[e]) : acc[e], acc[e + 1] = some ? fmaf(f, v.y, acc[e + 1]) : acc[e + 1];
       }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -989,7 +990,7 @@ int64_t seen_blocks(const AttendParams &A) {
 // Which units are cut, and into how many pieces; returns the time estimated, in
 // that of a block (2 us): a unit or piece takes its blocks and three more, and
 // a join about five.  (28/4 heads: 64 tokens at the end of 32K 544 us with
-// whole units, 75 cut; 4,096 tokens, 3.08 rounds of units, 1,989 and 1,592.)
+// whole units, 68 cut; 4,096 tokens, 3.08 rounds of units, 1,989 and 1,592.)
 // Tokens that are the greater part of their context see ever less towards the
 // first ones, which come last and even the ends out by themselves: 8,192 of 8K
 // (8/8 heads) took 166 us whole, 191 cut.
@@ -1050,7 +1051,10 @@ int run(PrefillParams &P, const CUtensorMap &tk, const CUtensorMap &tv, int32_t 
   prof_after(slot, st);
   const int s = launch_status();
   if (s != SB_OK || P.splits == 1) return s;
-  join_pieces_kernel<D><<<dim3((unsigned)(P.n_units - P.whole), kPieceRows / kJoinRows), kJoinThreads, 0, st>>>(P);
+  // A CTA takes 16 or 32 rows: few cut units want many CTAs, many want the unit found less often.  (64 tokens of
+  // 32K, 8 units: 69 us in all with 16 rows, 76 with 32; 8 requests of 8K and 64 tokens, 64 units: 121 and 110.)
+  const unsigned cut = (unsigned)(P.n_units - P.whole), parts = cut * 8 < (unsigned)sm_count() ? 16 : 8;
+  join_pieces_kernel<D><<<dim3(cut, parts), kJoinThreads, 0, st>>>(P);
   return launch_status();
 }
 
@@ -1132,9 +1136,9 @@ bool prefill_takes(const AttendParams &P, int dtype) {
   // 106 and 154)
   if ((int64_t)P.batch.n_tokens * P.G <= 16 * (int64_t)P.batch.batch) return false;
   // Estimates in us (codes: the expansion is the third term), fitted to 1 to 64 requests of 1K to 32K keys.
-  // 16-bit rows, the other path and this one: 1 x 32K keys, 4 tokens 43 and 48, 8 tokens 60 and 50, 64 tokens
-  // 333 and 75; 1 x 1K, 64 tokens 33 and 35; 8 x 8K, 4 tokens 61 and 62, 16 tokens 179 and 68; 64 x 1K, 2 tokens
-  // 37 and 54, 4 tokens 64 and 54.  Codes: 1 x 32K, 16 tokens 84 and 107, 32 tokens 148 and 113; 8 x 32K, 10
+  // 16-bit rows, the other path and this one: 1 x 32K keys, 4 tokens 43 and 48, 8 tokens 60 and 43, 64 tokens
+  // 333 and 68; 1 x 1K, 64 tokens 33 and 35; 8 x 8K, 4 tokens 61 and 62, 16 tokens 179 and 65; 64 x 1K, 2 tokens
+  // 37 and 54, 4 tokens 64 and 54.  Codes: 1 x 32K, 16 tokens 84 and 107, 32 tokens 148 and 100; 8 x 32K, 10
   // tokens 332 and 377, 16 tokens 516 and 381.
   const double blocks = (double)seen_blocks(P);
   PrefillParams Q;
